@@ -246,7 +246,7 @@ def _plain_recurrence(case, st):
         s_out = torch.where((length > 0)[:, None], h[rows, last], s)
         if not case["train"]:
             return [s_out, h.to(st["x"].dtype)]
-        g = st["gy"].float()
+        g = st["gy"].to(torch.float32, copy=True)
         g[rows, last] += torch.where((length > 0)[:, None], st["gs"], torch.zeros_like(st["gs"]))
         behind = torch.cat([kept[:, 1:], torch.zeros_like(kept[:, :1])], dim=1)
         dh = _scan(behind.flip(1), g.flip(1)).flip(1)

@@ -226,6 +226,61 @@ int b200wkv7_mix_post_bwd(void* stream, int dtype, long long rows, int H, int N,
                           const void* ln_w, const void* ln_b, const void* r_k, const void* gx,
                           void* dy, void* dr, void* dk, void* dv, void* dg, float* partial);
 
+/* ---------------------------------------------------- gated linear recurrence ----
+ * One number of state per channel (no counterpart in jaxrwkv), with the conventions of the recurrences above:
+ *   B200WKV_GATE_SIGMOID: a = sigmoid(f),     u = (1 - a) x
+ *   B200WKV_GATE_DECAY:   a = exp(-exp(f)),   u = x          (f: the raw log-log decay, as RWKV-7's w)
+ *   h_t = (start_t ? 0 : a_t h_{t-1}) + u_t,  y_t = h_t
+ * x, f, y and their gradients have element type `dtype`; states are fp32 in memory and in the arithmetic.  A sequence's tokens
+ * are rows of C adjacent channels: for x and f `*_batch` and `*_token` are the elements from sequence to sequence and from
+ * token to token, which may be halves of wider rows; y, gy, dx and df are dense (B, T, C), states dense (B, C).  Any C, any
+ * address that suits the element type.  s_out is the state after token length-1 (s0 when length == 0; length > T is T); y is
+ * computed for all T tokens.  A start flag drops the state in front of its token whatever it holds.  length NULL: T
+ * everywhere; new_starts NULL: none; s0 NULL: zeros.
+ *
+ * `residual` (b200wkv_gated_residual_bytes) is filled by the forward for the backward, which only reads it; NULL for
+ * inference.  gy or gs may be NULL (= zeros).  No output may overlap an input. */
+#define B200WKV_GATE_SIGMOID 0
+#define B200WKV_GATE_DECAY   1
+size_t b200wkv_gated_residual_bytes(int B, int T, int C);
+int b200wkv_gated_fwd(void* stream, int dtype, int gate, int B, int T, int C,
+                      const void* x, long long x_batch, long long x_token,
+                      const void* f, long long f_batch, long long f_token,
+                      const float* s0, const uint32_t* length, const uint8_t* new_starts,
+                      void* y, float* s_out, void* residual, size_t residual_bytes);
+int b200wkv_gated_bwd(void* stream, int dtype, int gate, int B, int T, int C,
+                      const void* x, long long x_batch, long long x_token,
+                      const void* f, long long f_batch, long long f_token,
+                      const uint32_t* length, const uint8_t* new_starts,
+                      const void* gy, const float* gs, const void* residual, size_t residual_bytes,
+                      void* dx, void* df, float* ds0);
+/* One token: rows of C channels, `*_stride` elements apart (y dense).  s_out may be s (the state is then updated where it
+ * lies).  A row of length 0 keeps its state and has its y all the same. */
+int b200wkv_gated_step(void* stream, int dtype, int gate, int B, int C, const void* x, long long x_stride,
+                       const void* f, long long f_stride, const float* s, long long s_stride,
+                       const uint32_t* length, const uint8_t* new_starts,
+                       void* y, float* s_out, long long s_out_stride);
+
+/* ------------------------------------------------- group norm with an activation ----
+ * The output stage of RWKV-5, 5.2 and 6 (jaxrwkv src/jaxrwkv/rwkv6.py: group norm, times silu of the gate stream) and of gated
+ * recurrences.  Rows of C channels, statistics per row and group of C / groups consecutive channels (at most 8192):
+ *   n = (x - mean) / sqrt(var + eps) * weight + bias,   y = act(n), or n * act(gate) where a gate is given
+ * x and gate: rows `*_stride` elements apart; y, gy, dx, dgate dense (rows, C); weight and bias (C,) of element type
+ * `param_dtype`, each or both NULL (ones, zeros).  Any address that suits the element types.  The backward computes the
+ * statistics again from x; dgate is needed exactly when there is a gate; dweight and dbias (of `param_dtype`) may be NULL, else
+ * `workspace` holds b200wkv_group_norm_workspace_bytes() of scratch, 4-byte aligned.  Deterministic: no atomics. */
+#define B200WKV_ACT_NONE    0
+#define B200WKV_ACT_SIGMOID 1
+#define B200WKV_ACT_SILU    2
+int b200wkv_group_norm_fwd(void* stream, int dtype, long long rows, int C, int groups, float eps, int activation,
+                           const void* x, long long x_stride, const void* weight, const void* bias, int param_dtype,
+                           const void* gate, long long gate_stride, void* y);
+size_t b200wkv_group_norm_workspace_bytes(long long rows, int C);
+int b200wkv_group_norm_bwd(void* stream, int dtype, long long rows, int C, int groups, float eps, int activation,
+                           const void* x, long long x_stride, const void* weight, const void* bias, int param_dtype,
+                           const void* gate, long long gate_stride, const void* gy,
+                           void* dx, void* dgate, void* dweight, void* dbias, void* workspace, size_t workspace_bytes);
+
 /* Forward + backward in one call with NO residual buffer from the caller (no counterpart in
  * jaxrwkv: its kernels always take the residuals as operands).
  *

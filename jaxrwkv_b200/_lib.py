@@ -16,6 +16,8 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
 _U = ctypes.c_uint
+_L = ctypes.c_longlong
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); must list every symbol the header declares
 PROTOTYPES = {
@@ -42,6 +44,13 @@ PROTOTYPES = {
     "b200wkv7_mix_pre_bwd": (_I, [_P, _I, ctypes.c_longlong, _I, _I, _I] + [_P] * 23),
     "b200wkv7_mix_post_fwd": (_I, [_P, _I, ctypes.c_longlong, _I, _I, ctypes.c_float] + [_P] * 9),
     "b200wkv7_mix_post_bwd": (_I, [_P, _I, ctypes.c_longlong, _I, _I, ctypes.c_float] + [_P] * 15),
+    "b200wkv_gated_residual_bytes": (_SZ, [_I, _I, _I]),
+    "b200wkv_gated_fwd": (_I, [_P] + [_I] * 5 + [_P, _L, _L] * 2 + [_P] * 3 + [_P] * 3 + [_SZ]),
+    "b200wkv_gated_bwd": (_I, [_P] + [_I] * 5 + [_P, _L, _L] * 2 + [_P] * 2 + [_P] * 3 + [_SZ] + [_P] * 3),
+    "b200wkv_gated_step": (_I, [_P] + [_I] * 4 + [_P, _L] * 3 + [_P] * 4 + [_L]),
+    "b200wkv_group_norm_fwd": (_I, [_P, _I, _L, _I, _I, _F, _I, _P, _L, _P, _P, _I, _P, _L, _P]),
+    "b200wkv_group_norm_workspace_bytes": (_SZ, [_L, _I]),
+    "b200wkv_group_norm_bwd": (_I, [_P, _I, _L, _I, _I, _F, _I, _P, _L, _P, _P, _I, _P, _L, _P] + [_P] * 5 + [_SZ]),
     "b200wkv7_static_scratch_bytes": (_SZ, []),
     "b200wkv7_fwd_bwd_static": (_I, [_P, _I, _I, _I, _I, _I] + [_P] * 9 + [_P, _P] + [_P, _P] + [_P] * 7 + [_U]),
 }

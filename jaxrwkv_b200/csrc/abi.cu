@@ -549,4 +549,95 @@ int b200wkv_token_shift_bwd(void* stream, int dtype, int B, int T, int D, int M,
                            gprev, gmix);
 }
 
+static bool known(int dtype) { return dtype == B200WKV_F32 || dtype == B200WKV_BF16; }
+static size_t element_bytes(int dtype) { return dtype == B200WKV_F32 ? 4 : 2; }
+
+// The tiles of a sequence are counted and the grid is made in 32 bits.
+static int check_gated(int dtype, int gate, int B, int T, int C) {
+    if (!known(dtype)) return B200WKV_EDTYPE;
+    if (gate != B200WKV_GATE_SIGMOID && gate != B200WKV_GATE_DECAY) return B200WKV_EUNSUPPORTED;
+    if (B < 1 || T < 1 || C < 1 || (long long)B * T > 2147483647LL || T > (1 << 30) || (long long)B * C > (1LL << 30)) return B200WKV_ESHAPE;
+    return B200WKV_OK;
+}
+
+size_t b200wkv_gated_residual_bytes(int B, int T, int C) {
+    return check_gated(B200WKV_F32, B200WKV_GATE_SIGMOID, B, T, C) == B200WKV_OK ? gated_residual_bytes(B, T, C) : 0;
+}
+
+int b200wkv_gated_fwd(void* stream, int dtype, int gate, int B, int T, int C, const void* x, long long x_batch, long long x_token,
+                      const void* f, long long f_batch, long long f_token, const float* s0, const uint32_t* length,
+                      const uint8_t* new_starts, void* y, float* s_out, void* residual, size_t residual_bytes) {
+    int st = check_gated(dtype, gate, B, T, C);
+    if (st != B200WKV_OK) return st;
+    if (!x || !f || !y || !s_out) return B200WKV_ENULL;
+    if (residual != nullptr && residual_bytes < gated_residual_bytes(B, T, C)) return B200WKV_ERESIDUAL;
+    if (!aligned(element_bytes(dtype), {x, f, y}) || !aligned(4, {s0, length, s_out, residual})) return B200WKV_EUNSUPPORTED;
+    if (T == 1 && residual == nullptr && s0 != nullptr)
+        return gated_step((cudaStream_t)stream, dtype, gate, B, C, x, x_batch, f, f_batch, s0, C, length, new_starts, y, s_out, C);
+    return gated_fwd((cudaStream_t)stream, dtype, gate, B, T, C, x, x_batch, x_token, f, f_batch, f_token, s0, length, new_starts, y, s_out,
+                     residual);
+}
+
+int b200wkv_gated_bwd(void* stream, int dtype, int gate, int B, int T, int C, const void* x, long long x_batch, long long x_token,
+                      const void* f, long long f_batch, long long f_token, const uint32_t* length, const uint8_t* new_starts,
+                      const void* gy, const float* gs, const void* residual, size_t residual_bytes, void* dx, void* df, float* ds0) {
+    int st = check_gated(dtype, gate, B, T, C);
+    if (st != B200WKV_OK) return st;
+    if (!x || !f || !residual || !dx || !df || !ds0) return B200WKV_ENULL;
+    if (residual_bytes < gated_residual_bytes(B, T, C)) return B200WKV_ERESIDUAL;
+    if (!aligned(element_bytes(dtype), {x, f, gy, dx, df}) || !aligned(4, {gs, length, residual, ds0})) return B200WKV_EUNSUPPORTED;
+    return gated_bwd((cudaStream_t)stream, dtype, gate, B, T, C, x, x_batch, x_token, f, f_batch, f_token, length, new_starts, gy, gs, residual,
+                     dx, df, ds0);
+}
+
+int b200wkv_gated_step(void* stream, int dtype, int gate, int B, int C, const void* x, long long x_stride, const void* f,
+                       long long f_stride, const float* s, long long s_stride, const uint32_t* length, const uint8_t* new_starts, void* y,
+                       float* s_out, long long s_out_stride) {
+    int st = check_gated(dtype, gate, B, 1, C);
+    if (st != B200WKV_OK) return st;
+    if (!x || !f || !s || !y || !s_out) return B200WKV_ENULL;
+    if (!aligned(element_bytes(dtype), {x, f, y}) || !aligned(4, {s, length, s_out})) return B200WKV_EUNSUPPORTED;
+    return gated_step((cudaStream_t)stream, dtype, gate, B, C, x, x_stride, f, f_stride, s, s_stride, length, new_starts, y, s_out, s_out_stride);
+}
+
+static int check_norm(int dtype, long long rows, int C, int groups, int activation, int param_dtype) {
+    if (!known(dtype) || !known(param_dtype)) return B200WKV_EDTYPE;
+    if (activation < B200WKV_ACT_NONE || activation > B200WKV_ACT_SILU) return B200WKV_EUNSUPPORTED;
+    if (rows < 1 || rows > 2147483647LL || C < 1 || C > (1 << 24) || groups < 1 || C % groups != 0 || C / groups > 8192) return B200WKV_ESHAPE;
+    return B200WKV_OK;
+}
+
+int b200wkv_group_norm_fwd(void* stream, int dtype, long long rows, int C, int groups, float eps, int activation, const void* x,
+                           long long x_stride, const void* weight, const void* bias, int param_dtype, const void* gate,
+                           long long gate_stride, void* y) {
+    int st = check_norm(dtype, rows, C, groups, activation, param_dtype);
+    if (st != B200WKV_OK) return st;
+    if (!x || !y) return B200WKV_ENULL;
+    if (!aligned(element_bytes(dtype), {x, gate, y}) || !aligned(element_bytes(param_dtype), {weight, bias})) return B200WKV_EUNSUPPORTED;
+    return group_norm_fwd((cudaStream_t)stream, dtype, rows, C, groups, eps, activation, x, x_stride, weight, bias, param_dtype, gate,
+                          gate_stride, y);
+}
+
+size_t b200wkv_group_norm_workspace_bytes(long long rows, int C) {
+    return check_norm(B200WKV_F32, rows, C, C, B200WKV_ACT_NONE, B200WKV_F32) == B200WKV_OK ? group_norm_workspace_bytes(rows, C) : 0;
+}
+
+int b200wkv_group_norm_bwd(void* stream, int dtype, long long rows, int C, int groups, float eps, int activation, const void* x,
+                           long long x_stride, const void* weight, const void* bias, int param_dtype, const void* gate,
+                           long long gate_stride, const void* gy, void* dx, void* dgate, void* dweight, void* dbias, void* workspace,
+                           size_t workspace_bytes) {
+    int st = check_norm(dtype, rows, C, groups, activation, param_dtype);
+    if (st != B200WKV_OK) return st;
+    if (!x || !gy || !dx || (gate == nullptr) != (dgate == nullptr)) return B200WKV_ENULL;
+    if (dweight != nullptr || dbias != nullptr) {
+        if (!workspace) return B200WKV_ENULL;
+        if (workspace_bytes < group_norm_workspace_bytes(rows, C)) return B200WKV_ERESIDUAL;
+    }
+    if (!aligned(element_bytes(dtype), {x, gate, gy, dx, dgate}) || !aligned(element_bytes(param_dtype), {weight, bias, dweight, dbias}) ||
+        !aligned(4, {workspace}))
+        return B200WKV_EUNSUPPORTED;
+    return group_norm_bwd((cudaStream_t)stream, dtype, rows, C, groups, eps, activation, x, x_stride, weight, bias, param_dtype, gate,
+                          gate_stride, gy, dx, dgate, dweight, dbias, workspace);
+}
+
 }  // extern "C"

@@ -72,4 +72,21 @@ struct PartialRows {
 };
 int column_sums(cudaStream_t st, int dtype, const PartialRows (&of)[3], void* out);
 
+// Gated linear recurrence, its step and the group norm behind the C ABI's checks.
+size_t gated_residual_bytes(int B, int T, int C);
+int gated_fwd(cudaStream_t st, int dtype, int gate, int B, int T, int C, const void* x, long long x_batch, long long x_token, const void* f,
+              long long f_batch, long long f_token, const float* s0, const uint32_t* length, const uint8_t* ns, void* y, float* s_out,
+              void* residual);
+int gated_bwd(cudaStream_t st, int dtype, int gate, int B, int T, int C, const void* x, long long x_batch, long long x_token, const void* f,
+              long long f_batch, long long f_token, const uint32_t* length, const uint8_t* ns, const void* gy, const float* gs,
+              const void* residual, void* dx, void* df, float* ds0);
+int gated_step(cudaStream_t st, int dtype, int gate, int B, int C, const void* x, long long x_stride, const void* f, long long f_stride,
+               const float* s, long long s_stride, const uint32_t* length, const uint8_t* ns, void* y, float* s_out, long long s_out_stride);
+size_t group_norm_workspace_bytes(long long rows, int C);
+int group_norm_fwd(cudaStream_t st, int dtype, long long rows, int C, int groups, float eps, int act, const void* x, long long x_stride,
+                   const void* weight, const void* bias, int param_dtype, const void* gate, long long gate_stride, void* y);
+int group_norm_bwd(cudaStream_t st, int dtype, long long rows, int C, int groups, float eps, int act, const void* x, long long x_stride,
+                   const void* weight, const void* bias, int param_dtype, const void* gate, long long gate_stride, const void* gy, void* dx,
+                   void* dgate, void* dweight, void* dbias, void* workspace);
+
 }  // namespace b200wkv

@@ -10,6 +10,7 @@
 #include <torch/csrc/python_headers.h>
 
 #include <array>
+#include <climits>
 #include <functional>
 #include <memory>
 #include <unordered_map>
@@ -108,21 +109,25 @@ bool sizes_are(const Tensor& t, at::IntArrayRef lead, std::initializer_list<int6
 }
 
 // `length` as (lead) 32-bit words and `new_starts` as (lead, T) bytes; both may be shared by leading axes.
+Tensor length_words(const Tensor& len, at::IntArrayRef lead, const Tensor& like) {
+    if (len.scalar_type() == at::kInt && len.device() == like.device() && len.sizes() == lead && len.is_contiguous()) return len;
+    return len.to(like.device()).expand(lead).to(at::kInt).contiguous();
+}
+Tensor start_bytes(const Tensor& ns, at::IntArrayRef shape, const Tensor& like) {
+    if ((ns.scalar_type() == at::kByte || ns.scalar_type() == at::kBool) && ns.device() == like.device() && ns.sizes() == shape &&
+        ns.is_contiguous())
+        return ns;
+    Tensor starts = ns.to(like.device());
+    if (starts.scalar_type() != at::kBool) starts = starts.to(at::kByte);
+    return starts.expand(shape).contiguous();
+}
 struct Flags {
     Tensor length, starts;
     Flags(const Tensor& len, const Tensor& ns, at::IntArrayRef lead, int64_t T, const Tensor& like) {
-        length = len;
-        if (!(len.scalar_type() == at::kInt && len.device() == like.device() && len.sizes() == lead && len.is_contiguous()))
-            length = len.to(like.device()).expand(lead).to(at::kInt).contiguous();
+        length = length_words(len, lead, like);
         std::vector<int64_t> shape(lead.begin(), lead.end());
         shape.push_back(T);
-        starts = ns;
-        if (!((ns.scalar_type() == at::kByte || ns.scalar_type() == at::kBool) && ns.device() == like.device() &&
-              ns.sizes() == at::IntArrayRef(shape) && ns.is_contiguous())) {
-            starts = ns.to(like.device());
-            if (starts.scalar_type() != at::kBool) starts = starts.to(at::kByte);
-            starts = starts.expand(shape).contiguous();
-        }
+        starts = start_bytes(ns, shape, like);
     }
 };
 
@@ -852,6 +857,194 @@ struct LayerNode : public torch::autograd::Function<LayerNode> {
     }
 };
 
+// ------------------------------------------------------------------------------------------------- gated linear recurrence
+// Rows of adjacent channels where the caller keeps them, as (n, C) or (B, T, C) with strides of their own.
+Tensor rows_of(const Tensor& t, at::IntArrayRef shape) {
+    const Tensor v = t.sizes() == shape ? t : t.reshape(shape);
+    return v.stride(-1) == 1 || v.size(-1) == 1 ? v : v.contiguous();
+}
+bool known_type(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
+bool beside(const Tensor& t, const Tensor& like) { return t.is_cuda() && t.device() == like.device() && t.layout() == at::kStrided; }
+
+// x, f (lead, T, C), state (lead, C) in fp32
+struct Gated {
+    static constexpr const char* kName = "gated_recurrence";
+    struct Dims {
+        at::IntArrayRef lead;
+        int64_t B, T, C;
+        explicit Dims(const Tensor& x) : lead(x.sizes().slice(0, x.dim() - 2)), B(c10::multiply_integers(lead)), T(x.size(-2)), C(x.size(-1)) {}
+    };
+    static bool fits(const Tensor* t) {
+        if (!same_kind(t, 2) || t[0].dim() < 2 || !t[1].sizes().equals(t[0].sizes())) return false;
+        const Dims d(t[0]);
+        return d.B * d.T <= INT_MAX && d.C <= INT_MAX && beside(t[2], t[0]) && t[2].scalar_type() == at::kFloat && sizes_are(t[2], d.lead, {d.C});
+    }
+    struct Flagged {
+        Tensor length, starts;
+        Flagged(const Tensor& len, const Tensor& ns, const Dims& d, const Tensor& like) {
+            if (len.defined()) length = length_words(len, d.lead, like);
+            if (!ns.defined()) return;
+            std::vector<int64_t> shape(d.lead.begin(), d.lead.end());
+            shape.push_back(d.T);
+            starts = start_bytes(ns, shape, like);
+        }
+    };
+    static std::pair<Tensor, Tensor> forward(int64_t gate, const Tensor* t, const Dims& d, const Flagged& f, Tensor* residual) {
+        const c10::cuda::CUDAGuard guard(t[0].device());
+        const Tensor x = rows_of(t[0], {d.B, d.T, d.C}), g = rows_of(t[1], {d.B, d.T, d.C}), s = t[2].contiguous();
+        Tensor y = fresh(t[0].sizes(), t[0].scalar_type(), t[0]), s_out = fresh(t[2].sizes(), at::kFloat, t[0]);
+        size_t rbytes = 0;
+        if (residual) {
+            rbytes = b200wkv_gated_residual_bytes((int)d.B, (int)d.T, (int)d.C);
+            *residual = bytes(rbytes, t[0]);
+        }
+        check(b200wkv_gated_fwd(stream_of(x), dtype_code(x), (int)gate, (int)d.B, (int)d.T, (int)d.C, in(x), x.stride(0), x.stride(1), in(g),
+                                g.stride(0), g.stride(1), (const float*)in(s), (const uint32_t*)in(f.length), (const uint8_t*)in(f.starts), out(y),
+                                (float*)out(s_out), residual ? out(*residual) : nullptr, rbytes));
+        return {s_out, y};
+    }
+    // saved: x f length new_starts residual; grads: of the returned state and of the output
+    static variable_list gradients(int64_t gate, const variable_list& saved, const variable_list& grads) {
+        const Dims d(saved[0]);
+        const c10::cuda::CUDAGuard guard(saved[0].device());
+        const Tensor x = rows_of(saved[0], {d.B, d.T, d.C}), g = rows_of(saved[1], {d.B, d.T, d.C}), &res = saved[4];
+        const Tensor gs = grads[0].defined() ? grads[0].to(at::kFloat).contiguous() : Tensor(), gy = cotangent(grads[1], x);
+        std::vector<int64_t> state(d.lead.begin(), d.lead.end());
+        state.push_back(d.C);
+        const Tensor dx = fresh(saved[0].sizes(), x.scalar_type(), x), df = fresh(saved[0].sizes(), x.scalar_type(), x), ds = fresh(state, at::kFloat, x);
+        check(b200wkv_gated_bwd(stream_of(x), dtype_code(x), (int)gate, (int)d.B, (int)d.T, (int)d.C, in(x), x.stride(0), x.stride(1), in(g),
+                                g.stride(0), g.stride(1), (const uint32_t*)in(saved[2]), (const uint8_t*)in(saved[3]), in(gy), (const float*)in(gs),
+                                in(res), (size_t)res.numel(), out(dx), out(df), (float*)out(ds)));
+        return {dx, df, ds};
+    }
+};
+struct GatedNode : public torch::autograd::Function<GatedNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& f, const Tensor& s, const Tensor& length,
+                                 const Tensor& starts, int64_t gate) {
+        const Tensor t[] = {x, f, s};
+        const Gated::Dims d(x);
+        const Gated::Flagged flagged(if_any(length), if_any(starts), d, x);
+        Tensor residual;
+        auto [s_out, y] = Gated::forward(gate, t, d, flagged, &residual);
+        ctx->save_for_backward({x, f, flagged.length, flagged.starts, residual});
+        ctx->saved_data["gate"] = gate;
+        ctx->set_materialize_grads(false);
+        return {s_out, y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const int64_t gate = ctx->saved_data["gate"].toInt();
+        variable_list g = once_differentiable(Gated::kName, saved, grads, [&]() { return Gated::gradients(gate, saved, grads); });
+        g.resize(6);
+        return g;
+    }
+};
+// One token: x, f, state (lead, C).  An undefined output when it does not fit.
+std::pair<Tensor, Tensor> gated_step(int64_t gate, const Tensor* t, const Tensor& length, const Tensor& starts, bool in_place) {
+    if (!same_kind(t, 2) || t[0].dim() < 1 || !t[1].sizes().equals(t[0].sizes()) || !beside(t[2], t[0]) || t[2].scalar_type() != at::kFloat ||
+        !t[2].sizes().equals(t[0].sizes()))
+        return {};
+    const int64_t C = t[0].size(-1), B = t[0].numel() / C;
+    if (B > INT_MAX || C > INT_MAX) return {};
+    const Tensor& s = t[2];
+    if (in_place && !(s.dim() == 2 && (s.stride(1) == 1 || C == 1) && (s.stride(0) >= C || B == 1)) && !s.is_contiguous()) return {};
+    const auto lead = t[0].sizes().slice(0, t[0].dim() - 1);
+    const c10::cuda::CUDAGuard guard(s.device());
+    const Tensor x = rows_of(t[0], {B, C}), f = rows_of(t[1], {B, C}), from = rows_of(s, {B, C});
+    const Tensor len = length.defined() ? length_words(length, lead, x) : length, 
+                 flags = starts.defined() && starts.dim() == (int64_t)lead.size() + 1 && starts.size(-1) == 1 ? starts.squeeze(-1) : starts,
+                 ns = flags.defined() ? start_bytes(flags, lead, x) : flags;
+    Tensor y = fresh(t[0].sizes(), x.scalar_type(), x), s_out = in_place ? s : fresh(s.sizes(), at::kFloat, x);
+    check(b200wkv_gated_step(stream_of(x), dtype_code(x), (int)gate, (int)B, (int)C, in(x), x.stride(0), in(f), f.stride(0), (const float*)in(from),
+                             from.stride(0), (const uint32_t*)in(len), (const uint8_t*)in(ns), out(y), (float*)out(s_out),
+                             in_place ? from.stride(0) : C));
+    if (in_place) torch::autograd::impl::bump_version(s);
+    return {s_out, y};
+}
+
+// ------------------------------------------------------------------------------------------------- group norm with an activation
+// x and gate (lead, C), weight and bias (C); weight, bias and gate may be missing
+struct Norm {
+    static constexpr const char* kName = "group_norm_act";
+    struct How {
+        int64_t groups, act;
+        double eps;
+    };
+    static int param_code(const Tensor* t) { return t[1].defined() ? dtype_code(t[1]) : t[2].defined() ? dtype_code(t[2]) : B200WKV_F32; }
+    // t: x weight bias gate
+    static bool fits(const Tensor* t) {
+        if (!same_kind(t, 1) || t[0].dim() < 1 || t[0].size(-1) > INT_MAX) return false;
+        for (int i : {1, 2})
+            if (t[i].defined() && !(beside(t[i], t[0]) && known_type(t[i]) && sizes_are(t[i], {}, {t[0].size(-1)}))) return false;
+        if (t[1].defined() && t[2].defined() && t[1].scalar_type() != t[2].scalar_type()) return false;
+        return !t[3].defined() || (beside(t[3], t[0]) && t[3].scalar_type() == t[0].scalar_type() && t[3].sizes().equals(t[0].sizes()));
+    }
+    struct Operands {
+        int64_t C, rows;
+        Tensor x, gate, weight, bias;
+        explicit Operands(const Tensor* t) : C(t[0].size(-1)), rows(t[0].numel() / C), x(rows_of(t[0], {rows, C})) {
+            if (t[3].defined()) gate = rows_of(t[3], {rows, C});
+            if (t[1].defined()) weight = t[1].contiguous();
+            if (t[2].defined()) bias = t[2].contiguous();
+        }
+    };
+    static Tensor forward(const How& how, const Tensor* t) {
+        const c10::cuda::CUDAGuard guard(t[0].device());
+        const Operands o(t);
+        Tensor y = fresh(t[0].sizes(), t[0].scalar_type(), t[0]);
+        check(b200wkv_group_norm_fwd(stream_of(o.x), dtype_code(o.x), o.rows, (int)o.C, (int)how.groups, (float)how.eps, (int)how.act, in(o.x),
+                                     o.x.stride(0), in(o.weight), in(o.bias), param_code(t), in(o.gate), o.gate.defined() ? o.gate.stride(0) : 0,
+                                     out(y)));
+        return y;
+    }
+    // saved: x weight bias gate; `wanted`: the same
+    static variable_list gradients(const How& how, const variable_list& saved, const variable_list& grads, const std::array<bool, 4>& wanted) {
+        if (!grads[0].defined()) return variable_list(4);
+        const c10::cuda::CUDAGuard guard(saved[0].device());
+        const Tensor* const t = saved.data();
+        const Operands o(t);
+        const Tensor gy = cotangent(grads[0], o.x);
+        variable_list g(4);
+        g[0] = fresh(t[0].sizes(), t[0].scalar_type(), t[0]);
+        if (o.gate.defined()) g[3] = fresh(t[0].sizes(), t[0].scalar_type(), t[0]);
+        for (int i : {1, 2})
+            if (t[i].defined() && wanted[i]) g[i] = fresh(t[i].sizes(), t[i].scalar_type(), t[0]);
+        const size_t wbytes = g[1].defined() || g[2].defined() ? b200wkv_group_norm_workspace_bytes(o.rows, (int)o.C) : 0;
+        const Tensor room = wbytes ? bytes(wbytes, t[0]) : Tensor();
+        check(b200wkv_group_norm_bwd(stream_of(o.x), dtype_code(o.x), o.rows, (int)o.C, (int)how.groups, (float)how.eps, (int)how.act, in(o.x),
+                                     o.x.stride(0), in(o.weight), in(o.bias), param_code(t), in(o.gate), o.gate.defined() ? o.gate.stride(0) : 0,
+                                     in(gy), out(g[0]), out(g[3]), out(g[1]), out(g[2]), out(room), wbytes));
+        return g;
+    }
+};
+struct NormNode : public torch::autograd::Function<NormNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& gate, int64_t groups,
+                          int64_t act, double eps) {
+        const Tensor t[] = {x, if_any(weight), if_any(bias), if_any(gate)};
+        ctx->save_for_backward({t[0], t[1], t[2], t[3]});
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["eps"] = eps;
+        ctx->set_materialize_grads(false);
+        return Norm::forward({groups, act, eps}, t);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Norm::How how{ctx->saved_data["groups"].toInt(), ctx->saved_data["act"].toInt(), ctx->saved_data["eps"].toDouble()};
+        std::array<bool, 4> wanted;
+        for (int i = 0; i < 4; ++i) wanted[i] = ctx->needs_input_grad(i);
+        variable_list g = once_differentiable(Norm::kName, saved, grads, [&]() {
+            variable_list all = Norm::gradients(how, saved, grads, wanted);
+            for (Tensor& one : all)
+                if (!one.defined()) one = nothing(saved[0]);       // (a node's results have to be defined)
+            return all;
+        });
+        for (Tensor& one : g) one = if_any(one);
+        g.resize(7);
+        return g;
+    }
+};
+
 // ------------------------------------------------------------------------------------------------- Python
 bool take(PyObject* const* args, int n, Tensor* to, bool look_for_tangents = true) {
     for (int i = 0; i < n; ++i) {
@@ -993,6 +1186,71 @@ PyObject* py_step_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {   // 
     END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_gated(PyObject*, PyObject* const* args, Py_ssize_t n) {   // (x, f, s, length, new_starts, gate)
+    HANDLE_TH_ERRORS
+    Tensor t[3], length, starts, s_out, y;
+    if (n != 6 || !take(args, 3, t) || !PyLong_CheckExact(args[5])) Py_RETURN_NONE;
+    if (args[3] != Py_None && !take(args + 3, 1, &length)) Py_RETURN_NONE;
+    if (args[4] != Py_None && !take(args + 4, 1, &starts)) Py_RETURN_NONE;
+    if (!Gated::fits(t)) Py_RETURN_NONE;
+    const int64_t gate = PyLong_AsLongLong(args[5]);
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (any_grad(t, 3)) {
+            variable_list o = GatedNode::apply(t[0], t[1], t[2], length.defined() ? length : nothing(t[0]), starts.defined() ? starts : nothing(t[0]), gate);
+            s_out = o[0]; y = o[1];
+        } else {
+            const Gated::Dims d(t[0]);
+            std::tie(s_out, y) = Gated::forward(gate, t, d, Gated::Flagged(length, starts, d, t[0]), nullptr);
+        }
+    }
+    return pair(s_out, y);
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_gated_step(PyObject*, PyObject* const* args, Py_ssize_t n) {   // (x, f, s, new_starts, length, gate, in place)
+    HANDLE_TH_ERRORS
+    Tensor t[3], length, starts, s_out, y;
+    if (n != 7 || !take(args, 3, t) || !PyLong_CheckExact(args[5])) Py_RETURN_NONE;
+    if (args[3] != Py_None && !take(args + 3, 1, &starts)) Py_RETURN_NONE;
+    if (args[4] != Py_None && !take(args + 4, 1, &length)) Py_RETURN_NONE;
+    const int64_t gate = PyLong_AsLongLong(args[5]);
+    if (any_grad(t, 3)) Py_RETURN_NONE;
+    {
+        pybind11::gil_scoped_release no_gil;
+        std::tie(s_out, y) = gated_step(gate, t, length, starts, args[6] == Py_True);
+    }
+    if (!y.defined()) Py_RETURN_NONE;
+    return pair(s_out, y);
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {   // (x, weight, bias, gate, groups, activation, eps)
+    HANDLE_TH_ERRORS
+    Tensor t[4], y;
+    if (n != 7 || !take(args, 1, t) || !PyLong_CheckExact(args[4]) || !PyLong_CheckExact(args[5]) || !PyFloat_CheckExact(args[6])) Py_RETURN_NONE;
+    for (int i = 1; i < 4; ++i)
+        if (args[i] != Py_None && !take(args + i, 1, t + i)) Py_RETURN_NONE;
+    if (!Norm::fits(t)) Py_RETURN_NONE;
+    const Norm::How how{PyLong_AsLongLong(args[4]), PyLong_AsLongLong(args[5]), PyFloat_AS_DOUBLE(args[6])};
+    if (how.groups < 1 || how.groups > t[0].size(-1)) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (any_grad(t, 1) || any_grad_defined(t + 1, 3)) {
+            for (int i = 1; i < 4; ++i)
+                if (!t[i].defined()) t[i] = nothing(t[0]);
+            y = NormNode::apply(t[0], t[1], t[2], t[3], how.groups, how.act, how.eps);
+        } else {
+            y = Norm::forward(how, t);
+        }
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_set_error_class(PyObject*, PyObject* cls) {
     Py_INCREF(cls);
     Py_XSETREF(g_error_class, cls);
@@ -1005,6 +1263,9 @@ PyMethodDef kMethods[] = {
     {"wkv4", (PyCFunction)(void (*)(void))py_wkv4, METH_FASTCALL, nullptr},
     {"time_mixing", (PyCFunction)(void (*)(void))py_time_mixing, METH_FASTCALL, nullptr},
     {"step_packed", (PyCFunction)(void (*)(void))py_step_packed, METH_FASTCALL, nullptr},
+    {"gated", (PyCFunction)(void (*)(void))py_gated, METH_FASTCALL, nullptr},
+    {"gated_step", (PyCFunction)(void (*)(void))py_gated_step, METH_FASTCALL, nullptr},
+    {"group_norm", (PyCFunction)(void (*)(void))py_group_norm, METH_FASTCALL, nullptr},
     {"set_error_class", py_set_error_class, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_b200wkv_host", "native host path of the WKV operators", -1, kMethods,

@@ -5,55 +5,48 @@
 // Both gates lie in [0, 1], so a product of them over any stretch of tokens cannot overflow.
 //
 // The recurrence is associative: a stretch of tokens acts on the state entering it as h -> A h + b.  A CTA of eight warps owns
-// 32 V channels of one sequence, each warp consecutive segments of kSeg tokens, and the CTAs of a cluster own consecutive tiles:
-//   1. every warp reduces its segment to (A, b), its gates staying in registers;
-//   2. these are combined in order, inside the CTA through shared memory and then across the cluster through distributed
-//      shared memory, which gives every segment the state entering it;
-//   3. every warp walks its segment from that state and writes the outputs.
-// The cluster then moves on by its tiles with the combined state as carry.
+// 64 channels of one sequence, a pair a lane, each warp consecutive segments of tokens, and the CTAs of a cluster own
+// consecutive tiles in turn:
+//   1. every warp turns its segment, which cp.async has brought into shared memory rounds ago, into gates and increments in
+//      registers, asks for the segment two rounds on, and reduces what it has to (A, b);
+//   2. the warps' (A, b) are combined in order through shared memory; where a cluster shares the sequence, the last warp sends
+//      the whole tile's to every CTA of it (st.async onto an mbarrier there), and everyone carries the state over all tiles of
+//      the round: one hop, whatever the size of the cluster;
+//   3. every warp walks its segment from the state that enters it and writes the outputs.
 //
 // Backward: dh_t = gy_t + [t == length-1] gs + c_{t+1},  c_t = start_t ? 0 : a_t dh_t.  The states are recomputed from the
-// state entering each tile, which the forward keeps (4 bytes per tile and channel); c runs over the segments from the last to
-// the first with the same products A.
+// state entering each tile of 64 tokens, which the forward keeps (4 bytes per 64 tokens and channel); c runs over the segments
+// from the last to the first with the same products A.
 //
 // A start flag cuts by a select, not by a factor of 0: what is no number in front of it ends there.
-#include <cooperative_groups.h>
-
 #include <initializer_list>
 
 #include "common.cuh"
 #include "device_once.cuh"
 #include "gate_math.cuh"
 #include "host_calls.h"
+#include "tc05.cuh"
 
 namespace b200wkv {
+int* wkv7_chunk_status_word();
 namespace {
-namespace cg = cooperative_groups;
+using namespace tc;
 
-constexpr int kSeg = 8;                    // tokens of a warp's segment
 constexpr int kWarps = 8;
-constexpr int kTile = kSeg * kWarps;       // tokens of a CTA's tile: a checkpoint each
+constexpr int kWide = 64;                  // channels of a CTA
+constexpr int kKept = 64;                  // tokens per kept state, and of a backward tile
 constexpr int kMaxCluster = 8;
+constexpr int kStages = 2;
+constexpr int kWaitRanOut = 3;             // status word: a wait for the other CTAs of a cluster
 
-// V channels, as they lie in memory
-template <typename T, int V> struct Raw;
-template <> struct Raw<float, 1> { float q; };
-template <> struct Raw<float, 2> { float2 q; };
-template <> struct Raw<__nv_bfloat16, 1> { __nv_bfloat16 q; };
-template <> struct Raw<__nv_bfloat16, 2> { uint32_t q; };
-__device__ __forceinline__ float channel(const Raw<float, 1>& r, int) { return r.q; }
-__device__ __forceinline__ float channel(const Raw<float, 2>& r, int v) { return v == 0 ? r.q.x : r.q.y; }
-__device__ __forceinline__ float channel(const Raw<__nv_bfloat16, 1>& r, int) { return __bfloat162float(r.q); }
-__device__ __forceinline__ float channel(const Raw<__nv_bfloat16, 2>& r, int v) { return __uint_as_float(v == 0 ? r.q << 16 : r.q & 0xffff0000u); }
-template <typename T, int V> __device__ __forceinline__ Raw<T, V> load_raw(const T* p) { return *reinterpret_cast<const Raw<T, V>*>(p); }
-template <int V> __device__ __forceinline__ void store_out(float* p, const float* h) {
-    if constexpr (V == 2) *reinterpret_cast<float2*>(p) = make_float2(h[0], h[1]);
-    else *p = h[0];
+// two channels, as they lie in shared memory
+__device__ __forceinline__ float2 pair_at(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 pair_at(const __nv_bfloat16* p) {
+    const uint32_t q = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(__uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
 }
-template <int V> __device__ __forceinline__ void store_out(__nv_bfloat16* p, const float* h) {
-    if constexpr (V == 2) *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(h[0], h[1]);
-    else *p = __float2bfloat16_rn(h[0]);
-}
+__device__ __forceinline__ void store_pair(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void store_pair(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
 
 constexpr int kSigmoidGate = B200WKV_GATE_SIGMOID;
 // The gate a, and what the backward needs of it: `w`, for the sigmoid 1 - a (to full relative precision), for the decay -da/df.
@@ -68,12 +61,6 @@ template <typename T, int kGate> __device__ __forceinline__ void gate_of(float f
     }
 }
 
-// start flags of the segment that begins at t0 as a bit mask (bit i = token t0 + i)
-__device__ __forceinline__ uint32_t segment_flags(const uint8_t* ns, int t0, int Tlen, int lane) {
-    const bool f = ns != nullptr && lane < kSeg && t0 + lane < Tlen && ns[t0 + lane] != 0;
-    return __ballot_sync(0xffffffffu, f);
-}
-
 struct Stream {                            // rows of C adjacent channels
     const void* p;
     long long batch, token;                // strides in elements
@@ -84,309 +71,390 @@ struct Problem {
     const float* s0;
     const uint32_t* length;
     const uint8_t* starts;
+    int* status;
 };
 
-// (A, b) of the segments and of the CTA; `cut`: a start flag lies inside
-template <int V> struct Summaries {
-    float A[kWarps][32 * V], b[kWarps][32 * V];
-    float cta_A[32 * V], cta_b[32 * V];
-    int cut[kWarps], cta_cut;
+// What a stretch does to the state of a channel: h -> A h + b.  A's sign bit says that a start flag lies inside: h is dropped.
+__device__ __forceinline__ bool cuts(float A) { return __float_as_int(A) < 0; }
+__device__ __forceinline__ float behind(float A, float b, float h) { return cuts(A) ? b : fmaf(A, h, b); }
+struct Stretch {
+    float4 v;                              // A, b of the lane's first channel, then of its second
+    __device__ __forceinline__ static Stretch nothing() { return {make_float4(1.f, 0.f, 1.f, 0.f)}; }
+    __device__ __forceinline__ void follow(float4 n) {               // by the stretch n
+        v.y = behind(n.x, n.y, v.y);
+        v.w = behind(n.z, n.w, v.w);
+        v.x = cuts(n.x) ? -1.f : v.x * n.x;
+        v.z = cuts(n.z) ? -1.f : v.z * n.z;
+    }
+    __device__ __forceinline__ float2 of(float2 h) const { return make_float2(behind(v.x, v.y, h.x), behind(v.z, v.w, h.y)); }
 };
 
-template <typename T, int V, int kGate>
-__global__ void __launch_bounds__(kWarps * 32, 2)
-gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, float* __restrict__ ckpt) {
-    __shared__ Summaries<V> sm;
-    const cg::cluster_group cluster = cg::this_cluster();
-    const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int unit = blockIdx.x / ranks, bi = unit / p.slabs, c = ((unit % p.slabs) * 32 + lane) * V;
-    const bool live = c < p.C;
-    const int cc = live ? c : 0;
-    const int L = p.length != nullptr ? (int)min(p.length[bi], (uint32_t)p.T) : p.T;
-    const int tiles = (p.T + kTile - 1) / kTile;
-    const size_t so = (size_t)bi * p.C + cc;
-    float carry[V];                        // state entering the tiles at hand
-#pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = p.s0 != nullptr ? p.s0[so + v] : 0.f;
-    if (L == 0 && warp == 0 && rank == 0 && live) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) s_out[so + v] = carry[v];
+// A warp's segments of one stream on their way to shared memory: kSeg rows of 64 channels, zeros behind the sequence's end and the
+// last channel.  Pieces of kPiece bytes; 2: single 16-bit elements, which no asynchronous copy takes.
+template <typename T, int kPiece, int kSeg> struct Feed {
+    static constexpr int kPer = kPiece / (int)sizeof(T), kPerRow = kWide / kPer;
+    static constexpr int kRows = kPerRow <= 32 ? 32 / kPerRow : 1, kPasses = kPerRow <= 32 ? 1 : kPerRow / 32;
+    const T* from;                         // the lane's first piece of token 0
+    long long stride;
+    int row, c, left;                      // the lane's first row and channel; channels that there are
+    __device__ __forceinline__ Feed(const void* p, long long batch, long long token, int bi, int c0, int C, int lane)
+        : stride(token), row(kPasses == 1 ? lane / kPerRow : 0), c((kPasses == 1 ? lane % kPerRow : lane) * kPer), left(C - c0) {
+        from = (const T*)p + bi * batch + c0;
     }
-    const T* const px = (const T*)p.x.p + bi * p.x.batch + cc;
-    const T* const pf = (const T*)p.f.p + bi * p.f.batch + cc;
-    T* const py = y + (size_t)bi * p.T * p.C + cc;
-    const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)bi * p.T : nullptr;
-    for (int tile0 = 0; tile0 < tiles; tile0 += ranks) {
-        const int tile = tile0 + rank, t0 = tile * kTile + warp * kSeg, n = max(0, min(kSeg, p.T - t0));
-        // 1. summary; tokens behind the end leave the state as it is
-        float a[kSeg][V], u[kSeg][V], A[V], b[V];
-        if (n > 0) {
-            Raw<T, V> rx[kSeg], rf[kSeg];
+    __device__ __forceinline__ void fetch(T* to, int t0, int Tlen) const {
 #pragma unroll
-            for (int i = 0; i < kSeg; ++i) {
-                const size_t t = (size_t)(t0 + min(i, n - 1));
-                rx[i] = load_raw<T, V>(px + t * p.x.token);
-                rf[i] = load_raw<T, V>(pf + t * p.f.token);
+        for (int i = 0; i < kSeg; i += kRows)
+#pragma unroll
+            for (int pass = 0; pass < kPasses; ++pass) {
+                const int t = t0 + i + row, ch = c + pass * 32 * kPer;
+                const bool valid = t < Tlen && ch < left;
+                const T* const at = from + (valid ? t * stride + ch : 0);
+                T* const dst = to + (i + row) * kWide + ch;
+                if constexpr (kPiece == 16) cp_async16(dst, at, valid);
+                else if constexpr (kPiece == 4)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(at), "r"(valid ? 4 : 0) : "memory");
+                else *dst = valid ? *at : from_f32<T>(0.f);
             }
-#pragma unroll
-            for (int i = 0; i < kSeg; ++i)
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    float w;
-                    gate_of<T, kGate>(channel(rf[i], v), a[i][v], w);
-                    u[i][v] = kGate == kSigmoidGate ? w * channel(rx[i], v) : channel(rx[i], v);
-                }
-        }
-        const uint32_t starts = segment_flags(ns, t0, p.T, lane);
-#pragma unroll
-        for (int v = 0; v < V; ++v) { A[v] = 1.f; b[v] = 0.f; }
-#pragma unroll
-        for (int i = 0; i < kSeg; ++i)
-            if (i < n) {
-                const bool start = (starts >> i) & 1u;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    b[v] = start ? u[i][v] : fmaf(a[i][v], b[v], u[i][v]);
-                    A[v] = start ? 0.f : A[v] * a[i][v];
-                }
-            }
-#pragma unroll
-        for (int v = 0; v < V; ++v) { sm.A[warp][lane * V + v] = A[v]; sm.b[warp][lane * V + v] = b[v]; }
-        if (lane == 0) sm.cut[warp] = starts != 0;
-        __syncthreads();
-        // 2. what the segments in front of this one make of the state entering the tile, and what the whole tile does
-        float qA[V], qb[V];
-        bool cut = false, own_cut = false;
-#pragma unroll
-        for (int v = 0; v < V; ++v) { qA[v] = 1.f; qb[v] = 0.f; }
-#pragma unroll
-        for (int j = 0; j < kWarps; ++j) {
-            if (j == warp) {
-                own_cut = cut;
-#pragma unroll
-                for (int v = 0; v < V; ++v) { A[v] = qA[v]; b[v] = qb[v]; }
-            }
-            const bool cj = sm.cut[j] != 0;
-            cut |= cj;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float Aj = sm.A[j][lane * V + v], bj = sm.b[j][lane * V + v];
-                qb[v] = cj ? bj : fmaf(Aj, qb[v], bj);
-                qA[v] = cj ? 0.f : Aj * qA[v];
-            }
-        }
-        if (ranks > 1) {
-            if (warp == 0) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) { sm.cta_A[lane * V + v] = qA[v]; sm.cta_b[lane * V + v] = qb[v]; }
-                if (lane == 0) sm.cta_cut = cut;
-            }
-            cluster.sync();
-        }
-        float h[V];
-        for (int q = 0; q < ranks; ++q) {
-            const bool own = q == rank;
-            const Summaries<V>* from = own ? &sm : cluster.map_shared_rank(&sm, q);
-            const bool cq = own ? cut : from->cta_cut != 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float Aq = own ? qA[v] : from->cta_A[lane * V + v], bq = own ? qb[v] : from->cta_b[lane * V + v];
-                if (own) h[v] = carry[v];
-                carry[v] = cq ? bq : fmaf(Aq, carry[v], bq);
-            }
-        }
-        if (ckpt != nullptr && warp == 0 && n > 0 && live) store_out<V>(ckpt + ((size_t)bi * tiles + tile) * p.C + cc, h);
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = own_cut ? b[v] : fmaf(A[v], h[v], b[v]);
-        // 3. outputs
-#pragma unroll
-        for (int i = 0; i < kSeg; ++i)
-            if (i < n) {
-                const bool start = (starts >> i) & 1u;
-#pragma unroll
-                for (int v = 0; v < V; ++v) h[v] = start ? u[i][v] : fmaf(a[i][v], h[v], u[i][v]);
-                if (live) {
-                    store_out<V>(py + (size_t)(t0 + i) * p.C, h);
-                    if (t0 + i == L - 1) store_out<V>(s_out + so, h);
-                }
-            }
-        if (ranks > 1) cluster.sync(); else __syncthreads();   // the summaries are read before the next ones are written
     }
+};
+__device__ __forceinline__ void fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void wait_fetched() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+    __syncwarp();
 }
 
-template <typename T, int V, int kGate>
+// A pair of channels of a dense row; single elements where pairs do not fit the row (kPiece one element) or its end
+template <typename T, int kPiece> __device__ __forceinline__ void put(T* p, float a, float b, int channels) {
+    if constexpr (kPiece >= 2 * (int)sizeof(T)) {
+        if (channels > 0) store_pair(p, a, b);
+    } else {
+        if (channels > 0) p[0] = from_f32<T>(a);
+        if (channels > 1) p[1] = from_f32<T>(b);
+    }
+}
+__device__ __forceinline__ float2 get_state(const float* p, int channels) {
+    return make_float2(p != nullptr && channels > 0 ? p[0] : 0.f, p != nullptr && channels > 1 ? p[1] : 0.f);
+}
+__device__ __forceinline__ void put_state(float* p, float2 h, int channels) {
+    if (channels > 0) p[0] = h.x;
+    if (channels > 1) p[1] = h.y;
+}
+
+// start flags of the kSeg tokens from t0 on as a bit mask (bit i = token t0 + i)
+template <int kSeg> __device__ __forceinline__ uint32_t segment_flags(const uint8_t* ns, int t0, int Tlen, int lane) {
+    if (ns == nullptr) return 0;
+    return __ballot_sync(0xffffffffu, lane < kSeg && t0 + lane < Tlen && ns[t0 + lane] != 0);
+}
+
+// What the CTAs of a cluster tell one another: the stretches of a round's tiles.  Two rounds' worth: a CTA sends a round's only when
+// it has those of the round in front from everyone, who by then have used the round before that.
+struct Exchange {
+    float4 tiles[2][kMaxCluster][32];
+    uint64_t bar[2];
+    __device__ __forceinline__ void open(int ranks) {
+        if (threadIdx.x == 0) {
+            mbar_init(&bar[0], 1);
+            mbar_init(&bar[1], 1);
+            mbar_init_fence();
+        }
+        if (ranks > 1) cluster_sync();
+    }
+    __device__ __forceinline__ void send(int round, int rank, int ranks, const Stretch& tile, int lane) {   // by one warp
+        uint64_t* const mine = &bar[round & 1];
+        if (lane == 0) mbar_expect_tx(mine, (uint32_t)ranks * 32 * sizeof(float4));
+        for (int q = 0; q < ranks; ++q) store_in_cta(in_cta(&tiles[round & 1][rank][lane], q), tile.v, in_cta(mine, q));
+    }
+    __device__ __forceinline__ void wait(int round, bool& lost, int* status) {
+        if (lost || mbar_wait_cluster(&bar[round & 1], (round >> 1) & 1)) return;
+        lost = true;
+        if (status != nullptr) *status = kWaitRanOut;
+    }
+    // no CTA leaves while others may still send to it
+    __device__ __forceinline__ void close(int ranks) { if (ranks > 1) cluster_sync(); }
+};
+
+struct Place {
+    int rank, ranks, lane, warp, bi, c, channels, L;
+    size_t state;                          // the lane's first channel in a dense (B, C) array
+    __device__ __forceinline__ Place(const Problem& p) {
+        rank = (int)cluster_rank(); ranks = (int)cluster_size();
+        lane = threadIdx.x & 31; warp = threadIdx.x >> 5;
+        const int unit = blockIdx.x / ranks;
+        bi = unit / p.slabs;
+        c = unit % p.slabs * kWide + 2 * lane;
+        channels = p.C - c;
+        L = p.length != nullptr ? (int)min(p.length[bi], (uint32_t)p.T) : p.T;
+        state = (size_t)bi * p.C + c;
+    }
+};
+struct Plain { static constexpr bool value = true; };      // a whole segment without a start flag in which the returned state is not taken
+struct Marked { static constexpr bool value = false; };
+
+template <typename T> constexpr int kFwdSeg = sizeof(T) == 2 ? 16 : 8;
+constexpr int kBwdSeg = kKept / kWarps;
+
+template <typename T, int kGate, int kPiece>
 __global__ void __launch_bounds__(kWarps * 32, 2)
-gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restrict__ gs, const float* __restrict__ ckpt,
-                 T* __restrict__ dx, T* __restrict__ df, float* __restrict__ ds0) {
-    __shared__ Summaries<V> sm;
-    __shared__ float back[kWarps][32 * V];     // what a segment sends to the one in front of it when nothing comes from behind
-    const cg::cluster_group cluster = cg::this_cluster();
-    const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int unit = blockIdx.x / ranks, bi = unit / p.slabs, c = ((unit % p.slabs) * 32 + lane) * V;
-    const bool live = c < p.C;
-    const int cc = live ? c : 0;
-    const int L = p.length != nullptr ? (int)min(p.length[bi], (uint32_t)p.T) : p.T;
-    const int tiles = (p.T + kTile - 1) / kTile;
-    const size_t so = (size_t)bi * p.C + cc, base = (size_t)bi * p.T * p.C + cc;
-    float carry[V], gstate[V];             // c entering the tiles at hand from behind; the returned state's cotangent
+gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, float* __restrict__ kept) {
+    constexpr int kSeg = kFwdSeg<T>, kTile = kSeg * kWarps, kHalf = kSeg * kWide;
+    extern __shared__ __align__(128) unsigned char dynamic[];
+    __shared__ Exchange ex;
+    __shared__ float4 segs[2][kWarps][32];
+    __shared__ float2 carried[2][32];
+    const Place at(p);
+    const int lane = at.lane, warp = at.warp, ranks = at.ranks, tiles = (p.T + kTile - 1) / kTile, rounds = (tiles + ranks - 1) / ranks;
+    const Feed<T, kPiece, kSeg> fx(p.x.p, p.x.batch, p.x.token, at.bi, at.c - 2 * lane, p.C, lane);
+    const Feed<T, kPiece, kSeg> ff(p.f.p, p.f.batch, p.f.token, at.bi, at.c - 2 * lane, p.C, lane);
+    T* const room = (T*)dynamic + warp * kStages * 2 * kHalf;
+    const auto first = [&](int round) { return (round * ranks + at.rank) * kTile + warp * kSeg; };
+    const auto ask = [&](int round) {
+        if (round < rounds) {
+            T* const to = room + round % kStages * 2 * kHalf;
+            fx.fetch(to, first(round), p.T);
+            ff.fetch(to + kHalf, first(round), p.T);
+        }
+        fetched();
+    };
+    for (int i = 0; i < kStages; ++i) ask(i);
+    float2 carry = get_state(p.s0 != nullptr ? p.s0 + at.state : nullptr, at.channels);      // state entering the round
+    if (at.L == 0 && warp == 0 && at.rank == 0) put_state(s_out + at.state, carry, at.channels);
+    if (warp == kWarps - 1) carried[0][lane] = carry;
+    ex.open(ranks);
+    bool lost = false;
+    T* const py = y + (size_t)at.bi * p.T * p.C + at.c;
+    const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)at.bi * p.T : nullptr;
+    for (int round = 0; round < rounds; ++round) {
+        const int t0 = first(round), n = max(0, min(kSeg, p.T - t0)), parity = round & 1;
+        const uint32_t starts = segment_flags<kSeg>(ns, t0, p.T, lane);
+        const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
+        // 1. gates and increments, and what the segment does
+        float a[kSeg][2], u[kSeg][2];
+        wait_fetched<kStages - 1>();
+        const T* const from = room + round % kStages * 2 * kHalf + 2 * lane;
 #pragma unroll
-    for (int v = 0; v < V; ++v) { carry[v] = 0.f; gstate[v] = gs != nullptr ? gs[so + v] : 0.f; }
-    const T* const px = (const T*)p.x.p + bi * p.x.batch + cc;
-    const T* const pf = (const T*)p.f.p + bi * p.f.batch + cc;
-    const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)bi * p.T : nullptr;
-    for (int tile0 = (tiles - 1) / ranks * ranks; tile0 >= 0; tile0 -= ranks) {
-        const int tile = tile0 + rank, t0 = tile * kTile + warp * kSeg, n = max(0, min(kSeg, p.T - t0));
-        float a[kSeg][V], w[kSeg][V], x[kSeg][V], g[kSeg][V], A[V], b[V], h[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = 0.f;
-        if (n > 0) {
-            Raw<T, V> rx[kSeg], rf[kSeg], rg[kSeg];
+        for (int i = 0; i < kSeg; ++i) {
+            const float2 x = pair_at(from + i * kWide), f = pair_at(from + kHalf + i * kWide);
+            float w0, w1;
+            gate_of<T, kGate>(f.x, a[i][0], w0);
+            gate_of<T, kGate>(f.y, a[i][1], w1);
+            u[i][0] = kGate == kSigmoidGate ? w0 * x.x : x.x;
+            u[i][1] = kGate == kSigmoidGate ? w1 * x.y : x.y;
+        }
+        __syncwarp();                      // the segment has been read
+        ask(round + kStages);
+        Stretch own = Stretch::nothing();
+        const auto summarise = [&](auto kind) {
 #pragma unroll
             for (int i = 0; i < kSeg; ++i) {
-                const size_t t = (size_t)(t0 + min(i, n - 1));
-                rx[i] = load_raw<T, V>(px + t * p.x.token);
-                rf[i] = load_raw<T, V>(pf + t * p.f.token);
-                if (gy != nullptr) rg[i] = load_raw<T, V>(gy + base + t * p.C);
-            }
-            const float* const q = ckpt + ((size_t)bi * tiles + tile) * p.C + cc;
-#pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = q[v];
-#pragma unroll
-            for (int i = 0; i < kSeg; ++i)
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    gate_of<T, kGate>(channel(rf[i], v), a[i][v], w[i][v]);
-                    x[i][v] = channel(rx[i], v);
-                    g[i][v] = gy != nullptr ? channel(rg[i], v) : 0.f;
-                    if (t0 + i == L - 1) g[i][v] += gstate[v];
+                if (!kind.value) {
+                    if (i >= n) { a[i][0] = a[i][1] = 1.f; u[i][0] = u[i][1] = 0.f; }
+                    if ((starts >> i) & 1u) { own.v = make_float4(-1.f, u[i][0], -1.f, u[i][1]); continue; }
                 }
-        }
-        const uint32_t starts = segment_flags(ns, t0, p.T, lane);
-        // 1. the segment's summary for the states, and what it sends to the front
-        float send[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) { A[v] = 1.f; b[v] = 0.f; send[v] = 0.f; }
-#pragma unroll
-        for (int i = 0; i < kSeg; ++i)
-            if (i < n) {
-                const bool start = (starts >> i) & 1u;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float u = kGate == kSigmoidGate ? w[i][v] * x[i][v] : x[i][v];
-                    b[v] = start ? u : fmaf(a[i][v], b[v], u);
-                    A[v] = start ? 0.f : A[v] * a[i][v];
-                }
+                own.v.y = fmaf(a[i][0], own.v.y, u[i][0]);
+                own.v.w = fmaf(a[i][1], own.v.w, u[i][1]);
+                own.v.x *= a[i][0];
+                own.v.z *= a[i][1];
             }
-#pragma unroll
-        for (int i = kSeg - 1; i >= 0; --i)
-            if (i < n) {
-                const bool start = (starts >> i) & 1u;
-#pragma unroll
-                for (int v = 0; v < V; ++v) send[v] = start ? 0.f : a[i][v] * (g[i][v] + send[v]);
-            }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            sm.A[warp][lane * V + v] = A[v];
-            sm.b[warp][lane * V + v] = b[v];
-            back[warp][lane * V + v] = send[v];
-        }
-        if (lane == 0) sm.cut[warp] = starts != 0;
+        };
+        if (plain) summarise(Plain()); else summarise(Marked());
+        segs[parity][warp][lane] = own.v;
         __syncthreads();
-        // 2. the state entering the segment; what comes to it from behind
+        // 2. the state that enters the segment
+        Stretch front = Stretch::nothing();
 #pragma unroll
         for (int j = 0; j < kWarps - 1; ++j)
-            if (j < warp) {
-                const bool cj = sm.cut[j] != 0;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float Aj = sm.A[j][lane * V + v], bj = sm.b[j][lane * V + v];
-                    h[v] = cj ? bj : fmaf(Aj, h[v], bj);
-                }
+            if (j < warp) front.follow(segs[parity][j][lane]);
+        float2 h;
+        if (ranks > 1) {
+            if (warp == kWarps - 1) {
+                Stretch tile = front;
+                tile.follow(own.v);
+                ex.send(round, at.rank, ranks, tile, lane);
             }
-        float qA[V], qb[V], from_behind[V];
-        bool cut = false, own_cut = false;
-#pragma unroll
-        for (int v = 0; v < V; ++v) { qA[v] = 1.f; qb[v] = 0.f; }
-#pragma unroll
-        for (int j = kWarps - 1; j >= 0; --j) {
-            if (j == warp) {
-                own_cut = cut;
-#pragma unroll
-                for (int v = 0; v < V; ++v) { A[v] = qA[v]; from_behind[v] = qb[v]; }
+            ex.wait(round, lost, p.status);
+            for (int q = 0; q < ranks; ++q) {
+                if (q == at.rank) h = carry;
+                const Stretch tile = {ex.tiles[parity][q][lane]};
+                carry = tile.of(carry);
             }
-            const bool cj = sm.cut[j] != 0;
-            cut |= cj;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float Aj = sm.A[j][lane * V + v], bj = back[j][lane * V + v];
-                qb[v] = cj ? bj : fmaf(Aj, qb[v], bj);
-                qA[v] = cj ? 0.f : Aj * qA[v];
-            }
+        } else {
+            h = carried[parity][lane];
         }
+        h = front.of(h);
+        // (a kept state is wanted in front of every 64th token; the returned one behind its token)
+        if (kept != nullptr && n > 0 && t0 % kKept == 0) put_state(kept + ((size_t)at.bi * ((p.T + kKept - 1) / kKept) + t0 / kKept) * p.C + at.c, h, at.channels);
+        // 3. outputs
+        const auto walk = [&](auto kind) {
+#pragma unroll
+            for (int i = 0; i < kSeg; ++i) {
+                const bool start = !kind.value && ((starts >> i) & 1u);
+                h.x = start ? u[i][0] : fmaf(a[i][0], h.x, u[i][0]);
+                h.y = start ? u[i][1] : fmaf(a[i][1], h.y, u[i][1]);
+                if (kind.value || i < n) put<T, kPiece>(py + (size_t)(t0 + i) * p.C, h.x, h.y, at.channels);
+                if (!kind.value && t0 + i == at.L - 1) put_state(s_out + at.state, h, at.channels);
+            }
+        };
+        if (plain) walk(Plain()); else walk(Marked());
+        if (ranks == 1 && warp == kWarps - 1) carried[parity ^ 1][lane] = h;
+    }
+    ex.close(ranks);
+}
+
+template <typename T, int kGate, int kPiece>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restrict__ gs, const float* __restrict__ kept,
+                 T* __restrict__ dx, T* __restrict__ df, float* __restrict__ ds0) {
+    constexpr int kSeg = kBwdSeg, kTile = kKept, kHalf = kSeg * kWide;
+    extern __shared__ __align__(128) unsigned char dynamic[];
+    __shared__ Exchange ex;
+    __shared__ float4 segs[2][kWarps][32];
+    __shared__ float2 sent[2][kWarps][32], carried[2][32];
+    const Place at(p);
+    const int lane = at.lane, warp = at.warp, ranks = at.ranks, tiles = (p.T + kTile - 1) / kTile, rounds = (tiles + ranks - 1) / ranks;
+    const Feed<T, kPiece, kSeg> fx(p.x.p, p.x.batch, p.x.token, at.bi, at.c - 2 * lane, p.C, lane);
+    const Feed<T, kPiece, kSeg> ff(p.f.p, p.f.batch, p.f.token, at.bi, at.c - 2 * lane, p.C, lane);
+    const Feed<T, kPiece, kSeg> fg(gy, (long long)p.T * p.C, p.C, at.bi, at.c - 2 * lane, p.C, lane);
+    T* const room = (T*)dynamic + warp * kStages * 3 * kHalf;
+    // rounds are taken from the last to the first; `done` of them lie behind
+    const auto first = [&](int done) { return ((rounds - 1 - done) * ranks + at.rank) * kTile + warp * kSeg; };
+    const auto ask = [&](int done) {
+        if (done < rounds) {
+            T* const to = room + done % kStages * 3 * kHalf;
+            fx.fetch(to, first(done), p.T);
+            ff.fetch(to + kHalf, first(done), p.T);
+            if (gy != nullptr) fg.fetch(to + 2 * kHalf, first(done), p.T);
+        }
+        fetched();
+    };
+    const auto entering = [&](int done) {  // the kept state in front of a round's tile
+        const int tile = (rounds - 1 - done) * ranks + at.rank;
+        return done < rounds && tile < tiles ? get_state(kept + ((size_t)at.bi * tiles + tile) * p.C + at.c, at.channels) : make_float2(0.f, 0.f);
+    };
+    for (int i = 0; i < kStages; ++i) ask(i);
+    float2 next = entering(0), carry = make_float2(0.f, 0.f);      // carry: c entering the round from behind
+    const float2 gstate = get_state(gs != nullptr ? gs + at.state : nullptr, at.channels);
+    if (warp == 0) carried[0][lane] = carry;
+    ex.open(ranks);
+    bool lost = false;
+    const size_t base = (size_t)at.bi * p.T * p.C + at.c;
+    const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)at.bi * p.T : nullptr;
+    for (int done = 0; done < rounds; ++done) {
+        const int t0 = first(done), n = max(0, min(kSeg, p.T - t0)), parity = done & 1;
+        const uint32_t starts = segment_flags<kSeg>(ns, t0, p.T, lane);
+        const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
+        float2 h = next;
+        next = entering(done + 1);
+        // 1. gates; what the segment does to the states, and what it sends to the front
+        float a[kSeg][2], w[kSeg][2], x[kSeg][2], g[kSeg][2];
+        wait_fetched<kStages - 1>();
+        const T* const from = room + done % kStages * 3 * kHalf + 2 * lane;
+#pragma unroll
+        for (int i = 0; i < kSeg; ++i) {
+            const float2 xi = pair_at(from + i * kWide), fi = pair_at(from + kHalf + i * kWide);
+            const float2 gi = gy != nullptr ? pair_at(from + 2 * kHalf + i * kWide) : make_float2(0.f, 0.f);
+            gate_of<T, kGate>(fi.x, a[i][0], w[i][0]);
+            gate_of<T, kGate>(fi.y, a[i][1], w[i][1]);
+            x[i][0] = xi.x; x[i][1] = xi.y;
+            g[i][0] = gi.x; g[i][1] = gi.y;
+        }
+        __syncwarp();                      // the segment has been read
+        ask(done + kStages);
+        const auto increment = [&](int i, int v) { return kGate == kSigmoidGate ? w[i][v] * x[i][v] : x[i][v]; };
+        Stretch own = Stretch::nothing();
+        float2 c = make_float2(0.f, 0.f);
+        const auto summarise = [&](auto kind) {
+#pragma unroll
+            for (int i = 0; i < kSeg; ++i) {
+                if (!kind.value) {
+                    if (i >= n) {
+                        a[i][0] = a[i][1] = 1.f;
+                        w[i][0] = w[i][1] = x[i][0] = x[i][1] = 0.f;
+                    }
+                    if (t0 + i == at.L - 1) { g[i][0] += gstate.x; g[i][1] += gstate.y; }
+                    if ((starts >> i) & 1u) { own.v = make_float4(-1.f, increment(i, 0), -1.f, increment(i, 1)); continue; }
+                }
+                own.v.y = fmaf(a[i][0], own.v.y, increment(i, 0));
+                own.v.w = fmaf(a[i][1], own.v.w, increment(i, 1));
+                own.v.x *= a[i][0];
+                own.v.z *= a[i][1];
+            }
+#pragma unroll
+            for (int i = kSeg - 1; i >= 0; --i) {
+                const bool start = !kind.value && ((starts >> i) & 1u);
+                c.x = start ? 0.f : a[i][0] * (g[i][0] + c.x);
+                c.y = start ? 0.f : a[i][1] * (g[i][1] + c.y);
+            }
+        };
+        if (plain) summarise(Plain()); else summarise(Marked());
+        segs[parity][warp][lane] = own.v;
+        sent[parity][warp][lane] = c;
+        __syncthreads();
+        // 2. the state that enters the segment, and c that enters it from behind
+#pragma unroll
+        for (int j = 0; j < kWarps - 1; ++j)
+            if (j < warp) h = Stretch{segs[parity][j][lane]}.of(h);
+        Stretch rear = Stretch::nothing();
+        const auto before = [&](int j) {
+            const float4 s = segs[parity][j][lane];
+            const float2 b = sent[parity][j][lane];
+            return make_float4(s.x, b.x, s.z, b.y);
+        };
+#pragma unroll
+        for (int j = kWarps - 1; j > 0; --j)
+            if (j > warp) rear.follow(before(j));
+        float2 e;
         if (ranks > 1) {
             if (warp == 0) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) { sm.cta_A[lane * V + v] = qA[v]; sm.cta_b[lane * V + v] = qb[v]; }
-                if (lane == 0) sm.cta_cut = cut;
+                Stretch tile = rear;
+                tile.follow(make_float4(own.v.x, c.x, own.v.z, c.y));
+                ex.send(done, at.rank, ranks, tile, lane);
             }
-            cluster.sync();
-        }
-        float e[V];
-        for (int q = ranks - 1; q >= 0; --q) {
-            const bool own = q == rank;
-            const Summaries<V>* from = own ? &sm : cluster.map_shared_rank(&sm, q);
-            const bool cq = own ? cut : from->cta_cut != 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float Aq = own ? qA[v] : from->cta_A[lane * V + v], bq = own ? qb[v] : from->cta_b[lane * V + v];
-                if (own) e[v] = carry[v];
-                carry[v] = cq ? bq : fmaf(Aq, carry[v], bq);
+            ex.wait(done, lost, p.status);
+            for (int q = ranks - 1; q >= 0; --q) {
+                if (q == at.rank) e = carry;
+                const Stretch tile = {ex.tiles[parity][q][lane]};
+                carry = tile.of(carry);
             }
+        } else {
+            e = carried[parity][lane];
         }
+        e = rear.of(e);
+        // 3. the states again, and in the place of x what df is dh times of; then back through the segment
+        const auto walk = [&](auto kind) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) e[v] = own_cut ? from_behind[v] : fmaf(A[v], e[v], from_behind[v]);
-        // 3. the states again, and in their place what df is dh times of; then back through the segment
+            for (int i = 0; i < kSeg; ++i) {
+                const bool start = !kind.value && ((starts >> i) & 1u);
 #pragma unroll
-        for (int i = 0; i < kSeg; ++i)
-            if (i < n) {
-                const bool start = (starts >> i) & 1u;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float before = start ? 0.f : h[v], xi = x[i][v];
-                    const float u = kGate == kSigmoidGate ? w[i][v] * xi : xi;
-                    h[v] = start ? u : fmaf(a[i][v], h[v], u);
-                    x[i][v] = kGate == kSigmoidGate ? (before - xi) * a[i][v] * w[i][v] : start ? 0.f : -before * w[i][v];
+                for (int v = 0; v < 2; ++v) {
+                    float& hv = v == 0 ? h.x : h.y;
+                    const float in = start ? 0.f : hv, xi = x[i][v], u = increment(i, v);
+                    hv = start ? u : fmaf(a[i][v], hv, u);
+                    x[i][v] = kGate == kSigmoidGate ? (in - xi) * (a[i][v] * w[i][v]) : start ? 0.f : -in * w[i][v];
                 }
             }
 #pragma unroll
-        for (int i = kSeg - 1; i >= 0; --i)
-            if (i < n) {
-                const bool start = (starts >> i) & 1u;
-                float ox[V], of[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float dh = g[i][v] + e[v];
-                    ox[v] = kGate == kSigmoidGate ? dh * w[i][v] : dh;
-                    of[v] = dh * x[i][v];
-                    e[v] = start ? 0.f : a[i][v] * dh;
+            for (int i = kSeg - 1; i >= 0; --i) {
+                const bool start = !kind.value && ((starts >> i) & 1u);
+                const float d0 = g[i][0] + e.x, d1 = g[i][1] + e.y;
+                if (kind.value || i < n) {
+                    const size_t to = base + (size_t)(t0 + i) * p.C;
+                    put<T, kPiece>(dx + to, kGate == kSigmoidGate ? d0 * w[i][0] : d0, kGate == kSigmoidGate ? d1 * w[i][1] : d1, at.channels);
+                    put<T, kPiece>(df + to, d0 * x[i][0], d1 * x[i][1], at.channels);
                 }
-                if (live) {
-                    store_out<V>(dx + base + (size_t)(t0 + i) * p.C, ox);
-                    store_out<V>(df + base + (size_t)(t0 + i) * p.C, of);
-                }
+                e.x = start ? 0.f : a[i][0] * d0;
+                e.y = start ? 0.f : a[i][1] * d1;
             }
-        if (tile == 0 && warp == 0 && live) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) ds0[so + v] = e[v] + (L == 0 ? gstate[v] : 0.f);
-        }
-        if (ranks > 1) cluster.sync(); else __syncthreads();   // the summaries are read before the next ones are written
+        };
+        if (plain) walk(Plain()); else walk(Marked());
+        if (t0 == 0) put_state(ds0 + at.state, at.L == 0 ? make_float2(e.x + gstate.x, e.y + gstate.y) : e, at.channels);
+        if (ranks == 1 && warp == 0) carried[parity ^ 1][lane] = e;
     }
+    ex.close(ranks);
 }
 
 // One token: out = h = (start ? 0 : a s) + u; rows of length 0 keep their state (and have their output all the same).  A thread's
 // V channels are read before they are written, so s_out may be s.
+template <typename T, int V> struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Few { T q[V]; };
 template <typename T, int V, int kGate>
 __global__ void __launch_bounds__(256)
 gated_step_kernel(int B, int C, const T* x, long long x_stride, const T* f, long long f_stride, const float* s, long long s_stride,
@@ -396,61 +464,68 @@ gated_step_kernel(int B, int C, const T* x, long long x_stride, const T* f, long
     if (at >= (long long)B * per_row) return;
     const int bi = (int)(at / per_row), c = (int)(at - (long long)bi * per_row) * V;
     const bool start = starts != nullptr && starts[bi] != 0, keep = length != nullptr && length[bi] == 0;
-    const Raw<T, V> rx = load_raw<T, V>(x + bi * x_stride + c), rf = load_raw<T, V>(f + bi * f_stride + c);
-    const Raw<float, V> rs = load_raw<float, V>(s + bi * s_stride + c);
-    float h[V], out[V];
+    const Few<T, V> rx = *(const Few<T, V>*)(x + bi * x_stride + c), rf = *(const Few<T, V>*)(f + bi * f_stride + c);
+    const Few<float, V> rs = *(const Few<float, V>*)(s + bi * s_stride + c);
+    Few<T, V> ry;
+    Few<float, V> rh;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         float a, w;
-        gate_of<T, kGate>(channel(rf, v), a, w);
-        const float u = kGate == kSigmoidGate ? w * channel(rx, v) : channel(rx, v);
-        out[v] = start ? u : fmaf(a, channel(rs, v), u);
-        h[v] = keep ? channel(rs, v) : out[v];
+        gate_of<T, kGate>(to_f32(rf.q[v]), a, w);
+        const float u = kGate == kSigmoidGate ? w * to_f32(rx.q[v]) : to_f32(rx.q[v]), out = start ? u : fmaf(a, rs.q[v], u);
+        ry.q[v] = from_f32<T>(out);
+        rh.q[v] = keep ? rs.q[v] : out;
     }
-    store_out<V>(y + (size_t)bi * C + c, out);
-    store_out<V>(s_out + bi * s_out_stride + c, h);
+    *(Few<T, V>*)(y + (size_t)bi * C + c) = ry;
+    *(Few<float, V>*)(s_out + bi * s_out_stride + c) = rh;
 }
 
-int cluster_size(int units, int tiles) {
+// CTAs of a cluster: as many as it takes to have two on every SM, no more than there are tiles.
+int ranks_of(int units, int tiles) {
     int n = 1;
     while (n < kMaxCluster && n < tiles && units * n < 2 * sm_count_of_current_device()) n *= 2;
     return n;
 }
 template <typename Kernel, typename... Args>
-int launch(Kernel kern, cudaStream_t st, int B, const Problem& p, Args... args) {
-    const int tiles = (p.T + kTile - 1) / kTile, ranks = cluster_size(B * p.slabs, tiles);
+int launch(DeviceOnce& once, Kernel kern, cudaStream_t st, int B, const Problem& p, int tile, size_t smem, Args... args) {
+    if (!once.ok([&]() { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); })) return B200WKV_ELAUNCH;
+    const int ranks = ranks_of(B * p.slabs, (p.T + tile - 1) / tile);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(B * p.slabs * ranks));
     cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, p, args...) == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
 }
-// Two channels at a time where the rows allow it.
-bool pairs(int C, size_t element, std::initializer_list<const void*> streams, std::initializer_list<const void*> states,
-           std::initializer_list<long long> strides) {
-    uintptr_t bits = 0, state_bits = 0;
-    long long odd = C;
+// The widest pieces that every row of these begins on.
+int piece_of(int C, int element, std::initializer_list<const void*> streams, std::initializer_list<long long> strides) {
+    uintptr_t bits = (uintptr_t)C * element;
     for (const void* q : streams) bits |= reinterpret_cast<uintptr_t>(q);
-    for (const void* q : states) state_bits |= reinterpret_cast<uintptr_t>(q);
-    for (long long s : strides) odd |= s;
-    return bits % (2 * element) == 0 && state_bits % 8 == 0 && odd % 2 == 0;
+    for (long long s : strides) bits |= (uintptr_t)s * element;
+    return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
 }
 
-template <typename T, int V, int kGate>
-int fwd(cudaStream_t st, int B, Problem p, void* y, float* s_out, float* ckpt) {
-    p.slabs = (p.C + 32 * V - 1) / (32 * V);
-    return launch(gated_fwd_kernel<T, V, kGate>, st, B, p, (T*)y, s_out, ckpt);
+template <typename T, int kGate, int kPiece> int fwd(cudaStream_t st, int B, const Problem& p, void* y, float* s_out, float* kept) {
+    static DeviceOnce once;
+    constexpr int kTile = kFwdSeg<T> * kWarps;
+    return launch(once, gated_fwd_kernel<T, kGate, kPiece>, st, B, p, kTile, (size_t)kStages * 2 * kTile * kWide * sizeof(T), (T*)y, s_out, kept);
 }
-template <typename T, int V, int kGate>
-int bwd(cudaStream_t st, int B, Problem p, const void* gy, const float* gs, const float* ckpt, void* dx, void* df, float* ds0) {
-    p.slabs = (p.C + 32 * V - 1) / (32 * V);
-    return launch(gated_bwd_kernel<T, V, kGate>, st, B, p, (const T*)gy, gs, ckpt, (T*)dx, (T*)df, ds0);
+template <typename T, int kGate, int kPiece>
+int bwd(cudaStream_t st, int B, const Problem& p, const void* gy, const float* gs, const float* kept, void* dx, void* df, float* ds0) {
+    static DeviceOnce once;
+    return launch(once, gated_bwd_kernel<T, kGate, kPiece>, st, B, p, kKept, (size_t)kStages * 3 * kKept * kWide * sizeof(T), (const T*)gy, gs, kept,
+                  (T*)dx, (T*)df, ds0);
 }
+// calls `go` with the element type, the gate and the piece as template arguments
+#define B200WKV_GATED_PIECE(go, T, piece, ...) \
+    (piece == 16 ? B200WKV_GATED_GATE(go, T, 16, __VA_ARGS__) : piece == 4 ? B200WKV_GATED_GATE(go, T, 4, __VA_ARGS__) : B200WKV_GATED_GATE(go, T, (int)sizeof(T), __VA_ARGS__))
+#define B200WKV_GATED_GATE(go, T, n, ...) (gate == B200WKV_GATE_SIGMOID ? go<T, 0, n>(__VA_ARGS__) : go<T, 1, n>(__VA_ARGS__))
+
 template <typename T, int V, int kGate>
 int step(cudaStream_t st, int B, int C, const Stream& x, const Stream& f, const float* s, long long s_stride, const uint32_t* length,
          const uint8_t* starts, void* y, float* s_out, long long s_out_stride) {
@@ -459,35 +534,39 @@ int step(cudaStream_t st, int B, int C, const Stream& x, const Stream& f, const 
         B, C, (const T*)x.p, x.batch, (const T*)f.p, f.batch, s, s_stride, length, starts, (T*)y, s_out, s_out_stride);
     return cudaGetLastError() == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
 }
-// calls `go` with the element type, the channels at a time and the gate as template arguments
-#define B200WKV_GATED(go, two, ...)                                                                                                  \
-    (dtype == B200WKV_F32 ? (two ? (gate == B200WKV_GATE_SIGMOID ? go<float, 2, 0>(__VA_ARGS__) : go<float, 2, 1>(__VA_ARGS__))          \
-                                 : (gate == B200WKV_GATE_SIGMOID ? go<float, 1, 0>(__VA_ARGS__) : go<float, 1, 1>(__VA_ARGS__)))         \
-                          : (two ? (gate == B200WKV_GATE_SIGMOID ? go<__nv_bfloat16, 2, 0>(__VA_ARGS__) : go<__nv_bfloat16, 2, 1>(__VA_ARGS__)) \
-                                 : (gate == B200WKV_GATE_SIGMOID ? go<__nv_bfloat16, 1, 0>(__VA_ARGS__) : go<__nv_bfloat16, 1, 1>(__VA_ARGS__))))
 }  // namespace
 
-size_t gated_residual_bytes(int B, int T, int C) { return (size_t)B * ((T + kTile - 1) / kTile) * C * sizeof(float); }
+size_t gated_residual_bytes(int B, int T, int C) { return (size_t)B * ((T + kKept - 1) / kKept) * C * sizeof(float); }
 
 int gated_fwd(cudaStream_t st, int dtype, int gate, int B, int T, int C, const void* x, long long x_batch, long long x_token, const void* f,
               long long f_batch, long long f_token, const float* s0, const uint32_t* length, const uint8_t* ns, void* y, float* s_out,
               void* residual) {
-    const Problem p = {T, C, 0, {x, x_batch, x_token}, {f, f_batch, f_token}, s0, length, ns};
-    const bool two = pairs(C, dtype == B200WKV_F32 ? 4 : 2, {x, f, y}, {s0, s_out, residual}, {x_batch, x_token, f_batch, f_token});
-    return B200WKV_GATED(fwd, two, st, B, p, y, s_out, (float*)residual);
+    const Problem p = {T, C, (C + kWide - 1) / kWide, {x, x_batch, x_token}, {f, f_batch, f_token}, s0, length, ns, wkv7_chunk_status_word()};
+    const int piece = piece_of(C, dtype == B200WKV_F32 ? 4 : 2, {x, f, y}, {x_batch, x_token, f_batch, f_token});
+    return dtype == B200WKV_F32 ? B200WKV_GATED_PIECE(fwd, float, piece, st, B, p, y, s_out, (float*)residual)
+                                : B200WKV_GATED_PIECE(fwd, __nv_bfloat16, piece, st, B, p, y, s_out, (float*)residual);
 }
 int gated_bwd(cudaStream_t st, int dtype, int gate, int B, int T, int C, const void* x, long long x_batch, long long x_token, const void* f,
               long long f_batch, long long f_token, const uint32_t* length, const uint8_t* ns, const void* gy, const float* gs,
               const void* residual, void* dx, void* df, float* ds0) {
-    const Problem p = {T, C, 0, {x, x_batch, x_token}, {f, f_batch, f_token}, nullptr, length, ns};
-    const bool two = pairs(C, dtype == B200WKV_F32 ? 4 : 2, {x, f, gy, dx, df}, {gs, residual, ds0}, {x_batch, x_token, f_batch, f_token});
-    return B200WKV_GATED(bwd, two, st, B, p, gy, gs, (const float*)residual, dx, df, ds0);
+    const Problem p = {T, C, (C + kWide - 1) / kWide, {x, x_batch, x_token}, {f, f_batch, f_token}, nullptr, length, ns, wkv7_chunk_status_word()};
+    const int piece = piece_of(C, dtype == B200WKV_F32 ? 4 : 2, {x, f, gy, dx, df}, {x_batch, x_token, f_batch, f_token});
+    return dtype == B200WKV_F32 ? B200WKV_GATED_PIECE(bwd, float, piece, st, B, p, gy, gs, (const float*)residual, dx, df, ds0)
+                                : B200WKV_GATED_PIECE(bwd, __nv_bfloat16, piece, st, B, p, gy, gs, (const float*)residual, dx, df, ds0);
 }
 int gated_step(cudaStream_t st, int dtype, int gate, int B, int C, const void* x, long long x_stride, const void* f, long long f_stride,
                const float* s, long long s_stride, const uint32_t* length, const uint8_t* ns, void* y, float* s_out, long long s_out_stride) {
-    const bool two = pairs(C, dtype == B200WKV_F32 ? 4 : 2, {x, f, y}, {s, s_out}, {x_stride, f_stride, s_stride, s_out_stride});
     const Stream sx = {x, x_stride, 0}, sf = {f, f_stride, 0};
-    return B200WKV_GATED(step, two, st, B, C, sx, sf, s, s_stride, length, ns, y, s_out, s_out_stride);
+    // four channels a thread where rows and addresses allow it
+    uintptr_t bits = (uintptr_t)C | (uintptr_t)x_stride | (uintptr_t)f_stride | (uintptr_t)s_stride | (uintptr_t)s_out_stride;
+    const size_t few = 4 * (dtype == B200WKV_F32 ? 4 : 2);
+    const bool four = bits % 4 == 0 && (uintptr_t)x % few == 0 && (uintptr_t)f % few == 0 && (uintptr_t)y % few == 0 && (uintptr_t)s % 16 == 0 &&
+                      (uintptr_t)s_out % 16 == 0;
+    const auto go = [&](auto fn) { return fn(st, B, C, sx, sf, s, s_stride, length, ns, y, s_out, s_out_stride); };
+    const bool sigmoid = gate == B200WKV_GATE_SIGMOID;
+    if (dtype == B200WKV_F32) return four ? (sigmoid ? go(step<float, 4, 0>) : go(step<float, 4, 1>)) : (sigmoid ? go(step<float, 1, 0>) : go(step<float, 1, 1>));
+    return four ? (sigmoid ? go(step<__nv_bfloat16, 4, 0>) : go(step<__nv_bfloat16, 4, 1>))
+                : (sigmoid ? go(step<__nv_bfloat16, 1, 0>) : go(step<__nv_bfloat16, 1, 1>));
 }
 
 }  // namespace b200wkv

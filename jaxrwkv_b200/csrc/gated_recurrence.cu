@@ -41,23 +41,21 @@ constexpr int kWaitRanOut = 3;             // status word: a wait for the other 
 
 // two channels, as they lie in shared memory
 __device__ __forceinline__ float2 pair_at(const float* p) { return *reinterpret_cast<const float2*>(p); }
-__device__ __forceinline__ float2 pair_at(const __nv_bfloat16* p) {
-    const uint32_t q = *reinterpret_cast<const uint32_t*>(p);
-    return make_float2(__uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
-}
+__device__ __forceinline__ float2 pair_at(const __nv_bfloat16* p) { return unpack_pair(*reinterpret_cast<const uint32_t*>(p)); }
 __device__ __forceinline__ void store_pair(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
 __device__ __forceinline__ void store_pair(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
 
 constexpr int kSigmoidGate = B200WKV_GATE_SIGMOID;
 // The gate a, and what the backward needs of it: `w`, for the sigmoid 1 - a (to full relative precision), for the decay -da/df.
-template <typename T, int kGate> __device__ __forceinline__ void gate_of(float f, float& a, float& w) {
+template <typename T, int kGate> __device__ __forceinline__ void gate_of(float2 f, float2& a, float2& w) {
     if (kGate == kSigmoidGate) {
         sigmoid_pair<T>(f, a, w);
     } else {
         // (accurate in 16 bits too: the state sums 1 / (1 - a) tokens, and an error of a is that much larger in it)
-        const float e = expf(f);
-        a = expf(-e);
-        w = a == 0.f ? 0.f : e * a;        // (e may be infinite then)
+        const float2 e = make_float2(expf(f.x), expf(f.y));
+        a = make_float2(expf(-e.x), expf(-e.y));
+        w = mul2(e, a);
+        w = make_float2(a.x == 0.f ? 0.f : w.x, a.y == 0.f ? 0.f : w.y);        // (e may be infinite then)
     }
 }
 
@@ -101,20 +99,30 @@ template <typename T, int kPiece, int kSeg> struct Feed {
         : stride(token), row(kPasses == 1 ? lane / kPerRow : 0), c((kPasses == 1 ? lane % kPerRow : lane) * kPer), left(C - c0) {
         from = (const T*)p + bi * batch + c0;
     }
+    __device__ __forceinline__ static void piece(T* to, const T* from, bool valid) {
+        if constexpr (kPiece == 16) cp_async16(to, from, valid);
+        else if constexpr (kPiece == 4)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(valid ? 4 : 0) : "memory");
+        else *to = valid ? *from : from_f32<T>(0.f);
+    }
     __device__ __forceinline__ void fetch(T* to, int t0, int Tlen) const {
+        to += row * kWide + c;
+        if (t0 + kSeg <= Tlen && left >= kWide) {
+            const T* at = from + (t0 + row) * stride + c;
 #pragma unroll
-        for (int i = 0; i < kSeg; i += kRows)
+            for (int i = 0; i < kSeg; i += kRows, at += kRows * stride)
 #pragma unroll
-            for (int pass = 0; pass < kPasses; ++pass) {
-                const int t = t0 + i + row, ch = c + pass * 32 * kPer;
-                const bool valid = t < Tlen && ch < left;
-                const T* const at = from + (valid ? t * stride + ch : 0);
-                T* const dst = to + (i + row) * kWide + ch;
-                if constexpr (kPiece == 16) cp_async16(dst, at, valid);
-                else if constexpr (kPiece == 4)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(at), "r"(valid ? 4 : 0) : "memory");
-                else *dst = valid ? *at : from_f32<T>(0.f);
-            }
+                for (int pass = 0; pass < kPasses; ++pass) piece(to + i * kWide + pass * 32 * kPer, at + pass * 32 * kPer, true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kSeg; i += kRows)
+#pragma unroll
+                for (int pass = 0; pass < kPasses; ++pass) {
+                    const int t = t0 + i + row, ch = c + pass * 32 * kPer;
+                    const bool valid = t < Tlen && ch < left;
+                    piece(to + i * kWide + pass * 32 * kPer, from + (valid ? t * stride + ch : 0), valid);
+                }
+        }
     }
 };
 __device__ __forceinline__ void fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -228,44 +236,41 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
         const uint32_t starts = segment_flags<kSeg>(ns, t0, p.T, lane);
         const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
         // 1. gates and increments, and what the segment does
-        float a[kSeg][2], u[kSeg][2];
+        float2 a[kSeg], u[kSeg];
         wait_fetched<kStages - 1>();
         const T* const from = room + round % kStages * 2 * kHalf + 2 * lane;
 #pragma unroll
         for (int i = 0; i < kSeg; ++i) {
-            const float2 x = pair_at(from + i * kWide), f = pair_at(from + kHalf + i * kWide);
-            float w0, w1;
-            gate_of<T, kGate>(f.x, a[i][0], w0);
-            gate_of<T, kGate>(f.y, a[i][1], w1);
-            u[i][0] = kGate == kSigmoidGate ? w0 * x.x : x.x;
-            u[i][1] = kGate == kSigmoidGate ? w1 * x.y : x.y;
+            const float2 x = pair_at(from + i * kWide);
+            float2 w;
+            gate_of<T, kGate>(pair_at(from + kHalf + i * kWide), a[i], w);
+            u[i] = kGate == kSigmoidGate ? mul2(w, x) : x;
         }
         __syncwarp();                      // the segment has been read
         ask(round + kStages);
-        Stretch own = Stretch::nothing();
+        float2 A = both(1.f), b = both(0.f);
         const auto summarise = [&](auto kind) {
 #pragma unroll
             for (int i = 0; i < kSeg; ++i) {
                 if (!kind.value) {
-                    if (i >= n) { a[i][0] = a[i][1] = 1.f; u[i][0] = u[i][1] = 0.f; }
-                    if ((starts >> i) & 1u) { own.v = make_float4(-1.f, u[i][0], -1.f, u[i][1]); continue; }
+                    if (i >= n) { a[i] = both(1.f); u[i] = both(0.f); }
+                    if ((starts >> i) & 1u) { A = both(-1.f); b = u[i]; continue; }
                 }
-                own.v.y = fmaf(a[i][0], own.v.y, u[i][0]);
-                own.v.w = fmaf(a[i][1], own.v.w, u[i][1]);
-                own.v.x *= a[i][0];
-                own.v.z *= a[i][1];
+                b = fma2(a[i], b, u[i]);
+                A = mul2(A, a[i]);
             }
         };
         if (plain) summarise(Plain()); else summarise(Marked());
+        const Stretch own = {make_float4(A.x, b.x, A.y, b.y)};
         segs[parity][warp][lane] = own.v;
         __syncthreads();
         // 2. the state that enters the segment
-        Stretch front = Stretch::nothing();
-#pragma unroll
-        for (int j = 0; j < kWarps - 1; ++j)
-            if (j < warp) front.follow(segs[parity][j][lane]);
         float2 h;
         if (ranks > 1) {
+            Stretch front = Stretch::nothing();
+#pragma unroll
+            for (int j = 0; j < kWarps - 1; ++j)
+                if (j < warp) front.follow(segs[parity][j][lane]);
             if (warp == kWarps - 1) {
                 Stretch tile = front;
                 tile.follow(own.v);
@@ -277,20 +282,23 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
                 const Stretch tile = {ex.tiles[parity][q][lane]};
                 carry = tile.of(carry);
             }
+            h = front.of(h);
         } else {
             h = carried[parity][lane];
+#pragma unroll
+            for (int j = 0; j < kWarps - 1; ++j)
+                if (j < warp) h = Stretch{segs[parity][j][lane]}.of(h);
         }
-        h = front.of(h);
         // (a kept state is wanted in front of every 64th token; the returned one behind its token)
         if (kept != nullptr && n > 0 && t0 % kKept == 0) put_state(kept + ((size_t)at.bi * ((p.T + kKept - 1) / kKept) + t0 / kKept) * p.C + at.c, h, at.channels);
         // 3. outputs
+        T* to = py + (size_t)t0 * p.C;
         const auto walk = [&](auto kind) {
 #pragma unroll
-            for (int i = 0; i < kSeg; ++i) {
+            for (int i = 0; i < kSeg; ++i, to += p.C) {
                 const bool start = !kind.value && ((starts >> i) & 1u);
-                h.x = start ? u[i][0] : fmaf(a[i][0], h.x, u[i][0]);
-                h.y = start ? u[i][1] : fmaf(a[i][1], h.y, u[i][1]);
-                if (kind.value || i < n) put<T, kPiece>(py + (size_t)(t0 + i) * p.C, h.x, h.y, at.channels);
+                h = start ? u[i] : fma2(a[i], h, u[i]);
+                if (kind.value || i < n) put<T, kPiece>(to, h.x, h.y, at.channels);
                 if (!kind.value && t0 + i == at.L - 1) put_state(s_out + at.state, h, at.channels);
             }
         };
@@ -345,47 +353,35 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
         float2 h = next;
         next = entering(done + 1);
         // 1. gates; what the segment does to the states, and what it sends to the front
-        float a[kSeg][2], w[kSeg][2], x[kSeg][2], g[kSeg][2];
+        float2 a[kSeg], w[kSeg], x[kSeg], g[kSeg];
         wait_fetched<kStages - 1>();
         const T* const from = room + done % kStages * 3 * kHalf + 2 * lane;
 #pragma unroll
         for (int i = 0; i < kSeg; ++i) {
-            const float2 xi = pair_at(from + i * kWide), fi = pair_at(from + kHalf + i * kWide);
-            const float2 gi = gy != nullptr ? pair_at(from + 2 * kHalf + i * kWide) : make_float2(0.f, 0.f);
-            gate_of<T, kGate>(fi.x, a[i][0], w[i][0]);
-            gate_of<T, kGate>(fi.y, a[i][1], w[i][1]);
-            x[i][0] = xi.x; x[i][1] = xi.y;
-            g[i][0] = gi.x; g[i][1] = gi.y;
+            x[i] = pair_at(from + i * kWide);
+            gate_of<T, kGate>(pair_at(from + kHalf + i * kWide), a[i], w[i]);
+            g[i] = gy != nullptr ? pair_at(from + 2 * kHalf + i * kWide) : both(0.f);
         }
         __syncwarp();                      // the segment has been read
         ask(done + kStages);
-        const auto increment = [&](int i, int v) { return kGate == kSigmoidGate ? w[i][v] * x[i][v] : x[i][v]; };
-        Stretch own = Stretch::nothing();
-        float2 c = make_float2(0.f, 0.f);
+        const auto increment = [&](int i) { return kGate == kSigmoidGate ? mul2(w[i], x[i]) : x[i]; };
+        float2 A = both(1.f), b = both(0.f), c = both(0.f);
         const auto summarise = [&](auto kind) {
 #pragma unroll
             for (int i = 0; i < kSeg; ++i) {
                 if (!kind.value) {
-                    if (i >= n) {
-                        a[i][0] = a[i][1] = 1.f;
-                        w[i][0] = w[i][1] = x[i][0] = x[i][1] = 0.f;
-                    }
-                    if (t0 + i == at.L - 1) { g[i][0] += gstate.x; g[i][1] += gstate.y; }
-                    if ((starts >> i) & 1u) { own.v = make_float4(-1.f, increment(i, 0), -1.f, increment(i, 1)); continue; }
+                    if (i >= n) { a[i] = both(1.f); w[i] = x[i] = both(0.f); }
+                    if (t0 + i == at.L - 1) g[i] = add2(g[i], gstate);
+                    if ((starts >> i) & 1u) { A = both(-1.f); b = increment(i); continue; }
                 }
-                own.v.y = fmaf(a[i][0], own.v.y, increment(i, 0));
-                own.v.w = fmaf(a[i][1], own.v.w, increment(i, 1));
-                own.v.x *= a[i][0];
-                own.v.z *= a[i][1];
+                b = fma2(a[i], b, increment(i));
+                A = mul2(A, a[i]);
             }
 #pragma unroll
-            for (int i = kSeg - 1; i >= 0; --i) {
-                const bool start = !kind.value && ((starts >> i) & 1u);
-                c.x = start ? 0.f : a[i][0] * (g[i][0] + c.x);
-                c.y = start ? 0.f : a[i][1] * (g[i][1] + c.y);
-            }
+            for (int i = kSeg - 1; i >= 0; --i) c = !kind.value && ((starts >> i) & 1u) ? both(0.f) : mul2(a[i], add2(g[i], c));
         };
         if (plain) summarise(Plain()); else summarise(Marked());
+        const Stretch own = {make_float4(A.x, b.x, A.y, b.y)};
         segs[parity][warp][lane] = own.v;
         sent[parity][warp][lane] = c;
         __syncthreads();
@@ -393,17 +389,17 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
 #pragma unroll
         for (int j = 0; j < kWarps - 1; ++j)
             if (j < warp) h = Stretch{segs[parity][j][lane]}.of(h);
-        Stretch rear = Stretch::nothing();
         const auto before = [&](int j) {
             const float4 s = segs[parity][j][lane];
             const float2 b = sent[parity][j][lane];
             return make_float4(s.x, b.x, s.z, b.y);
         };
-#pragma unroll
-        for (int j = kWarps - 1; j > 0; --j)
-            if (j > warp) rear.follow(before(j));
         float2 e;
         if (ranks > 1) {
+            Stretch rear = Stretch::nothing();
+#pragma unroll
+            for (int j = kWarps - 1; j > 0; --j)
+                if (j > warp) rear.follow(before(j));
             if (warp == 0) {
                 Stretch tile = rear;
                 tile.follow(make_float4(own.v.x, c.x, own.v.z, c.y));
@@ -415,34 +411,33 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
                 const Stretch tile = {ex.tiles[parity][q][lane]};
                 carry = tile.of(carry);
             }
+            e = rear.of(e);
         } else {
             e = carried[parity][lane];
+#pragma unroll
+            for (int j = kWarps - 1; j > 0; --j)
+                if (j > warp) e = Stretch{before(j)}.of(e);
         }
-        e = rear.of(e);
-        // 3. the states again, and in the place of x what df is dh times of; then back through the segment
+        // 3. the states again, and in the place of x what df is dx times of; then back through the segment
         const auto walk = [&](auto kind) {
 #pragma unroll
             for (int i = 0; i < kSeg; ++i) {
                 const bool start = !kind.value && ((starts >> i) & 1u);
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    float& hv = v == 0 ? h.x : h.y;
-                    const float in = start ? 0.f : hv, xi = x[i][v], u = increment(i, v);
-                    hv = start ? u : fmaf(a[i][v], hv, u);
-                    x[i][v] = kGate == kSigmoidGate ? (in - xi) * (a[i][v] * w[i][v]) : start ? 0.f : -in * w[i][v];
-                }
+                const float2 in = start ? both(0.f) : h, u = increment(i);
+                h = start ? u : fma2(a[i], h, u);
+                if (kGate == kSigmoidGate) x[i] = mul2(fma2(x[i], both(-1.f), in), a[i]);
+                else x[i] = start ? both(0.f) : mul2(mul2(in, w[i]), both(-1.f));
             }
+            const size_t last = base + (size_t)(t0 + kSeg - 1) * p.C;
+            T *to_x = dx + last, *to_f = df + last;
 #pragma unroll
-            for (int i = kSeg - 1; i >= 0; --i) {
-                const bool start = !kind.value && ((starts >> i) & 1u);
-                const float d0 = g[i][0] + e.x, d1 = g[i][1] + e.y;
+            for (int i = kSeg - 1; i >= 0; --i, to_x -= p.C, to_f -= p.C) {
+                const float2 d = add2(g[i], e), o = kGate == kSigmoidGate ? mul2(d, w[i]) : d, of = mul2(o, x[i]);
                 if (kind.value || i < n) {
-                    const size_t to = base + (size_t)(t0 + i) * p.C;
-                    put<T, kPiece>(dx + to, kGate == kSigmoidGate ? d0 * w[i][0] : d0, kGate == kSigmoidGate ? d1 * w[i][1] : d1, at.channels);
-                    put<T, kPiece>(df + to, d0 * x[i][0], d1 * x[i][1], at.channels);
+                    put<T, kPiece>(to_x, o.x, o.y, at.channels);
+                    put<T, kPiece>(to_f, of.x, of.y, at.channels);
                 }
-                e.x = start ? 0.f : a[i][0] * d0;
-                e.y = start ? 0.f : a[i][1] * d1;
+                e = !kind.value && ((starts >> i) & 1u) ? both(0.f) : mul2(a[i], d);
             }
         };
         if (plain) walk(Plain()); else walk(Marked());
@@ -469,12 +464,16 @@ gated_step_kernel(int B, int C, const T* x, long long x_stride, const T* f, long
     Few<T, V> ry;
     Few<float, V> rh;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float a, w;
-        gate_of<T, kGate>(to_f32(rf.q[v]), a, w);
-        const float u = kGate == kSigmoidGate ? w * to_f32(rx.q[v]) : to_f32(rx.q[v]), out = start ? u : fmaf(a, rs.q[v], u);
-        ry.q[v] = from_f32<T>(out);
-        rh.q[v] = keep ? rs.q[v] : out;
+    for (int v = 0; v < V; v += 2) {
+        const int v1 = v + (V > 1);        // (one channel: twice the same)
+        const float2 x2 = make_float2(to_f32(rx.q[v]), to_f32(rx.q[v1])), s2 = make_float2(rs.q[v], rs.q[v1]);
+        float2 a, w;
+        gate_of<T, kGate>(make_float2(to_f32(rf.q[v]), to_f32(rf.q[v1])), a, w);
+        const float2 u = kGate == kSigmoidGate ? mul2(w, x2) : x2, out = start ? u : fma2(a, s2, u);
+        ry.q[v] = from_f32<T>(out.x);
+        ry.q[v1] = from_f32<T>(out.y);
+        rh.q[v] = keep ? s2.x : out.x;
+        rh.q[v1] = keep ? s2.y : out.y;
     }
     *(Few<T, V>*)(y + (size_t)bi * C + c) = ry;
     *(Few<float, V>*)(s_out + bi * s_out_stride + c) = rh;

@@ -27,8 +27,33 @@ constexpr int kMaxThreads = 1024;
 struct Params {                            // weight or bias; p NULL: ones or zeros
     const void* p;
     int f32;
-    __device__ __forceinline__ float at(int c, float otherwise) const {
-        return p == nullptr ? otherwise : f32 ? ((const float*)p)[c] : __bfloat162float(((const __nv_bfloat16*)p)[c]);
+    // N from the c-th on, as pairs (N == 1: the same in both places); 16-byte loads where `vectors`
+    template <int N> __device__ __forceinline__ void load(int c, bool vectors, float otherwise, float2* to) const {
+        if (p == nullptr) {
+#pragma unroll
+            for (int i = 0; i < (N + 1) / 2; ++i) to[i] = both(otherwise);
+        } else if constexpr (N == 1) {
+            to[0] = both(f32 ? ((const float*)p)[c] : __bfloat162float(((const __nv_bfloat16*)p)[c]));
+        } else if (f32 && vectors) {
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) {
+                const float4 q = ((const float4*)((const float*)p + c))[i];
+                to[2 * i] = make_float2(q.x, q.y);
+                to[2 * i + 1] = make_float2(q.z, q.w);
+            }
+        } else if (vectors) {
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) {
+                const uint2 q = ((const uint2*)((const __nv_bfloat16*)p + c))[i];
+                to[2 * i] = unpack_pair(q.x);
+                to[2 * i + 1] = unpack_pair(q.y);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i)
+                to[i] = f32 ? make_float2(((const float*)p)[c + 2 * i], ((const float*)p)[c + 2 * i + 1])
+                            : make_float2(__bfloat162float(((const __nv_bfloat16*)p)[c + 2 * i]), __bfloat162float(((const __nv_bfloat16*)p)[c + 2 * i + 1]));
+        }
     }
 };
 struct Problem {
@@ -41,63 +66,60 @@ struct Problem {
     int team;                              // threads of a team
     int per_cta;                           // teams at work in a CTA: all of them, or a multiple of G
     int parallel;                          // rows at a time over the grid
+    int param_vectors;                     // weight and bias begin on 16 bytes
     int reduce;                            // teams of one group within a CTA are added up (per_cta is a multiple of G)
 };
 
-template <typename T, int VEC> __device__ __forceinline__ void load_piece(const T* p, float* v) {
-    if constexpr (VEC == 1) {
-        v[0] = to_f32(*p);
-    } else if constexpr (sizeof(T) == 4) {
-        const float4 q = *reinterpret_cast<const float4*>(p);
-        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+// A piece of a row as it lies in memory: VEC elements, 16 bytes, or one.  As pairs of floats a single element stands in both places.
+template <typename T, int VEC> struct Piece { uint4 q; };
+template <typename T> struct Piece<T, 1> { T q; };
+template <typename T, int VEC> __device__ __forceinline__ void unpack(const Piece<T, VEC>& r, float2* v) {
+    if constexpr (VEC == 1) v[0] = both(to_f32(r.q));
+    else if constexpr (sizeof(T) == 4) {
+        v[0] = make_float2(__uint_as_float(r.q.x), __uint_as_float(r.q.y));
+        v[1] = make_float2(__uint_as_float(r.q.z), __uint_as_float(r.q.w));
     } else {
-        const uint4 q = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+        v[0] = unpack_pair(r.q.x); v[1] = unpack_pair(r.q.y); v[2] = unpack_pair(r.q.z); v[3] = unpack_pair(r.q.w);
     }
 }
-template <typename T, int VEC> __device__ __forceinline__ void store_piece(T* p, const float* v) {
+template <typename T, int VEC> __device__ __forceinline__ void store_piece(T* p, const float2* v) {
     if constexpr (VEC == 1) {
-        *p = from_f32<T>(v[0]);
+        *p = from_f32<T>(v[0].x);
     } else if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
     } else {
         uint4 q;
         __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[i].x, v[i].y);
         *reinterpret_cast<uint4*>(p) = q;
     }
 }
+template <int VEC> __device__ __forceinline__ float sum_of(float2 v) { return VEC == 1 ? v.x : v.x + v.y; }
 
-// act(z) and its derivative
-template <typename T> __device__ __forceinline__ void activate(int act, float z, float& p, float& dp) {
-    if (act == B200WKV_ACT_NONE) { p = z; dp = 1.f; return; }
-    float s, r;
+// act(z), and its derivative where it is asked for
+template <typename T, int kAct> __device__ __forceinline__ void activate(float2 z, float2& p, float2& dp) {
+    if (kAct == B200WKV_ACT_NONE) { p = z; dp = both(1.f); return; }
+    float2 s, r;
     sigmoid_pair<T>(z, s, r);
-    p = act == B200WKV_ACT_SIGMOID ? s : z * s;
-    dp = act == B200WKV_ACT_SIGMOID ? s * r : s * fmaf(z, r, 1.f);
+    p = kAct == B200WKV_ACT_SIGMOID ? s : mul2(z, s);
+    dp = kAct == B200WKV_ACT_SIGMOID ? mul2(s, r) : mul2(s, fma2(z, r, both(1.f)));
 }
 
-// sums of two numbers over the team, the same in every thread of it
-template <bool kBlock> __device__ __forceinline__ void team_sum(float& a, float& b, int team, float2* room) {
-    const int width = kBlock ? 32 : team;
-    for (int o = width / 2; o > 0; o /= 2) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
+// sum over the team, the same in every thread of it
+template <bool kBlock> __device__ __forceinline__ float team_sum(float a, int team, float* room) {
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2)
+        if (kBlock || team > o) a += __shfl_xor_sync(0xffffffffu, a, o);
     if (kBlock) {
         const int warps = blockDim.x / 32;
         __syncthreads();                   // the last sums have been read
-        if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = make_float2(a, b);
+        if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = a;
         __syncthreads();
-        a = 0.f; b = 0.f;
-        for (int w = 0; w < warps; ++w) { a += room[w].x; b += room[w].y; }
+        a = 0.f;
+        for (int w = 0; w < warps; ++w) a += room[w];
     }
+    return a;
 }
 
 // Where a thread's team works: group g, rows first, first + parallel, ...; none of them where `at_work` is false
@@ -114,160 +136,194 @@ struct Place {
     }
 };
 
+// Registers: weight, bias and a row's values; 4 CTAs an SM where the team is a part of a warp
 template <typename T, int VEC, int K, bool kBlock, bool kGate>
-__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256)
+__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : VEC * K > 8 || VEC == 1 && K == 8 ? 2 : 4)
 group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
-    __shared__ float2 room[kBlock ? 32 : 1];
+    constexpr int kPairs = (VEC + 1) / 2;
+    __shared__ float room[kBlock ? 32 : 1];
     const Place at(p);
-    const int pieces = p.D / VEC, c0 = at.g * p.D;
+    const int pieces = p.D / VEC, c = at.g * p.D + at.lane * VEC, step = p.team * VEC;      // channels from piece to piece
     const float inv_d = 1.f / (float)p.D;
-    float w[K][VEC], b[K][VEC];
+    float2 w[K][kPairs], b[K][kPairs];
+    Piece<T, VEC> rx[K] = {}, rg[K] = {};
+    bool there[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+        there[k] = at.at_work && at.lane + k * p.team < pieces;
+        if (there[k]) {
+            p.weight.load<VEC>(c + k * step, p.param_vectors, 1.f, w[k]);
+            p.bias.load<VEC>(c + k * step, p.param_vectors, 0.f, b[k]);
+        } else {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const int d = (at.lane + k * p.team) * VEC + v;
-            w[k][v] = d < p.D ? p.weight.at(c0 + d, 1.f) : 0.f;
-            b[k][v] = d < p.D ? p.bias.at(c0 + d, 0.f) : 0.f;
+            for (int i = 0; i < kPairs; ++i) w[k][i] = b[k][i] = both(0.f);
         }
-    // (teams without work go along: the sums take whole warps and CTAs)
-    const long long steps = (p.rows + p.parallel - 1) / p.parallel;
-    for (long long i = 0; i < steps; ++i) {
-        const long long row = at.first + i * p.parallel;
-        const bool on = at.at_work && row < p.rows;
-        const T* const px = (const T*)p.x + row * p.x_stride + c0;
-        const T* const pg = (const T*)p.gate + row * p.gate_stride + c0;
-        float x[K][VEC], g[K][VEC], sum = 0.f, squares = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int piece = at.lane + k * p.team;
-            if (on && piece < pieces) {
-                load_piece<T, VEC>(px + piece * VEC, x[k]);
-                if (kGate) load_piece<T, VEC>(pg + piece * VEC, g[k]);
-            } else {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) x[k][v] = g[k][v] = 0.f;
-            }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) sum += x[k][v];
-        }
-        team_sum<kBlock>(sum, squares, p.team, room);
-        const float mean = sum * inv_d;
-        squares = 0.f;
+    }
+    const T* px = (const T*)p.x + at.first * p.x_stride + c;
+    const T* pg = kGate ? (const T*)p.gate + at.first * p.gate_stride + c : nullptr;
+    T* py = y + at.first * p.C + c;
+    const auto read = [&](long long row) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                x[k][v] -= mean;
-                if (at.lane + k * p.team < pieces) squares = fmaf(x[k][v], x[k][v], squares);
+            if (there[k] && row < p.rows) {
+                rx[k] = *(const Piece<T, VEC>*)(px + k * step);
+                if (kGate) rg[k] = *(const Piece<T, VEC>*)(pg + k * step);
             }
-        team_sum<kBlock>(squares, sum, p.team, room);
-        const float rstd = 1.f / sqrtf(squares * inv_d + p.eps);
-        T* const py = y + row * p.C + c0;
+        px += p.parallel * p.x_stride;
+        if (kGate) pg += p.parallel * p.gate_stride;
+    };
+    read(at.first);
+    // (teams without work go along: the sums take whole warps and CTAs)
+    const long long steps = (p.rows + p.parallel - 1) / p.parallel;
+    long long row = at.first;
+    for (long long i = 0; i < steps; ++i, row += p.parallel, py += (long long)p.parallel * p.C) {
+        float2 x[K][kPairs], g[K][kPairs], sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int piece = at.lane + k * p.team;
-            if (!on || piece >= pieces) continue;
-            float out[VEC];
+            unpack<T, VEC>(rx[k], x[k]);
+            if (kGate) unpack<T, VEC>(rg[k], g[k]);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float n = fmaf(x[k][v] * rstd, w[k][v], b[k][v]);
-                float a, da;
-                activate<T>(p.act, kGate ? g[k][v] : n, a, da);
-                out[v] = kGate ? n * a : a;
-            }
-            store_piece<T, VEC>(py + piece * VEC, out);
+            for (int j = 0; j < kPairs; ++j) sums = add2(sums, x[k][j]);
         }
+        read(row + p.parallel);
+        const float mean = team_sum<kBlock>(sum_of<VEC>(sums), p.team, room) * inv_d;
+        sums = both(0.f);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float2 squares = both(0.f);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+                x[k][j] = add2(x[k][j], both(-mean));
+                squares = fma2(x[k][j], x[k][j], squares);
+            }
+            if (there[k]) sums = add2(sums, squares);
+        }
+        const float rstd = rsqrtf(team_sum<kBlock>(sum_of<VEC>(sums), p.team, room) * inv_d + p.eps);
+        const auto finish = [&](auto act) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!there[k] || row >= p.rows) continue;
+                float2 out[kPairs];
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    const float2 n = fma2(mul2(x[k][j], both(rstd)), w[k][j], b[k][j]);
+                    float2 a, da;
+                    activate<T, act.value>(kGate ? g[k][j] : n, a, da);
+                    out[j] = kGate ? mul2(n, a) : a;
+                }
+                store_piece<T, VEC>(py + k * step, out);
+            }
+        };
+        if (p.act == B200WKV_ACT_SILU) finish(std::integral_constant<int, B200WKV_ACT_SILU>());
+        else if (p.act == B200WKV_ACT_SIGMOID) finish(std::integral_constant<int, B200WKV_ACT_SIGMOID>());
+        else finish(std::integral_constant<int, B200WKV_ACT_NONE>());
     }
 }
 
 template <typename T, int VEC, int K, bool kBlock, bool kGate>
-__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256)
+__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : VEC * K > 8 || VEC == 1 && K == 8 ? 1 : 2)
 group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ partial) {
-    __shared__ float2 room[kBlock ? 32 : 1];
-    __shared__ float both[kBlock ? 1 : 256 * VEC];
+    constexpr int kPairs = (VEC + 1) / 2;
+    __shared__ float room[kBlock ? 32 : 1];
+    __shared__ float both_sums[kBlock ? 1 : 256 * VEC];
     const Place at(p);
-    const int pieces = p.D / VEC, c0 = at.g * p.D;
+    const int pieces = p.D / VEC, c = at.g * p.D + at.lane * VEC, step = p.team * VEC;
     const float inv_d = 1.f / (float)p.D;
-    float w[K][VEC], b[K][VEC], dw[K][VEC], db[K][VEC];
+    float2 w[K][kPairs], b[K][kPairs], dw[K][kPairs], db[K][kPairs];
+    Piece<T, VEC> rx[K] = {}, rg[K] = {}, rd[K] = {};
+    bool there[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+        there[k] = at.at_work && at.lane + k * p.team < pieces;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const int d = (at.lane + k * p.team) * VEC + v;
-            w[k][v] = d < p.D ? p.weight.at(c0 + d, 1.f) : 0.f;
-            b[k][v] = d < p.D ? p.bias.at(c0 + d, 0.f) : 0.f;
-            dw[k][v] = db[k][v] = 0.f;
+        for (int i = 0; i < kPairs; ++i) w[k][i] = b[k][i] = dw[k][i] = db[k][i] = both(0.f);
+        if (there[k]) {
+            p.weight.load<VEC>(c + k * step, p.param_vectors, 1.f, w[k]);
+            p.bias.load<VEC>(c + k * step, p.param_vectors, 0.f, b[k]);
         }
-    const long long steps = (p.rows + p.parallel - 1) / p.parallel;
-    for (long long i = 0; i < steps; ++i) {
-        const long long row = at.first + i * p.parallel;
-        const bool on = at.at_work && row < p.rows;
-        const T* const px = (const T*)p.x + row * p.x_stride + c0;
-        const T* const pg = (const T*)p.gate + row * p.gate_stride + c0;
-        const size_t dense = (size_t)row * p.C + c0;
-        float x[K][VEC], g[K][VEC], d[K][VEC], sum = 0.f, other = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int piece = at.lane + k * p.team;
-            if (on && piece < pieces) {
-                load_piece<T, VEC>(px + piece * VEC, x[k]);
-                load_piece<T, VEC>(gy + dense + piece * VEC, d[k]);
-                if (kGate) load_piece<T, VEC>(pg + piece * VEC, g[k]);
-            } else {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) x[k][v] = g[k][v] = d[k][v] = 0.f;
-            }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) sum += x[k][v];
-        }
-        team_sum<kBlock>(sum, other, p.team, room);
-        const float mean = sum * inv_d;
-        float squares = 0.f;
+    }
+    const T* px = (const T*)p.x + at.first * p.x_stride + c;
+    const T* pg = kGate ? (const T*)p.gate + at.first * p.gate_stride + c : nullptr;
+    const T* pd = gy + at.first * p.C + c;
+    long long dense = at.first * p.C + c;
+    const auto read = [&](long long row) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                x[k][v] -= mean;
-                if (at.lane + k * p.team < pieces) squares = fmaf(x[k][v], x[k][v], squares);
+            if (there[k] && row < p.rows) {
+                rx[k] = *(const Piece<T, VEC>*)(px + k * step);
+                rd[k] = *(const Piece<T, VEC>*)(pd + k * step);
+                if (kGate) rg[k] = *(const Piece<T, VEC>*)(pg + k * step);
             }
-        team_sum<kBlock>(squares, other, p.team, room);
-        const float rstd = 1.f / sqrtf(squares * inv_d + p.eps);
-        float s1 = 0.f, s2 = 0.f;          // of dxh and dxh xh
+        px += p.parallel * p.x_stride;
+        pd += (long long)p.parallel * p.C;
+        if (kGate) pg += p.parallel * p.gate_stride;
+    };
+    read(at.first);
+    const long long steps = (p.rows + p.parallel - 1) / p.parallel;
+    long long row = at.first;
+    for (long long i = 0; i < steps; ++i, row += p.parallel, dense += (long long)p.parallel * p.C) {
+        const bool on = row < p.rows;
+        float2 x[K][kPairs], g[K][kPairs], d[K][kPairs], sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int piece = at.lane + k * p.team;
-            if (!on || piece >= pieces) continue;
+            unpack<T, VEC>(rx[k], x[k]);
+            unpack<T, VEC>(rd[k], d[k]);
+            if (kGate) unpack<T, VEC>(rg[k], g[k]);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float xh = x[k][v] * rstd, n = fmaf(xh, w[k][v], b[k][v]);
-                float a, da;
-                activate<T>(p.act, kGate ? g[k][v] : n, a, da);
-                const float dn = d[k][v] * (kGate ? a : da);
-                if (kGate) g[k][v] = d[k][v] * n * da;
-                dw[k][v] = fmaf(dn, xh, dw[k][v]);
-                db[k][v] += dn;
-                const float dxh = dn * w[k][v];
-                s1 += dxh;
-                s2 = fmaf(dxh, xh, s2);
-                x[k][v] = xh;
-                d[k][v] = dxh;
-            }
+            for (int j = 0; j < kPairs; ++j) sums = add2(sums, x[k][j]);
         }
-        team_sum<kBlock>(s1, s2, p.team, room);
-        s1 *= inv_d; s2 *= inv_d;
+        read(row + p.parallel);
+        const float mean = team_sum<kBlock>(sum_of<VEC>(sums), p.team, room) * inv_d;
+        sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int piece = at.lane + k * p.team;
-            if (!on || piece >= pieces) continue;
-            if (kGate) store_piece<T, VEC>(dgate + dense + piece * VEC, g[k]);
+            float2 squares = both(0.f);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) d[k][v] = rstd * (d[k][v] - s1 - x[k][v] * s2);
-            store_piece<T, VEC>(dx + dense + piece * VEC, d[k]);
+            for (int j = 0; j < kPairs; ++j) {
+                x[k][j] = add2(x[k][j], both(-mean));
+                squares = fma2(x[k][j], x[k][j], squares);
+            }
+            if (there[k]) sums = add2(sums, squares);
+        }
+        const float rstd = rsqrtf(team_sum<kBlock>(sum_of<VEC>(sums), p.team, room) * inv_d + p.eps);
+        float2 s1 = both(0.f), s2 = both(0.f);          // of dxh and dxh xh
+        const auto gradients = [&](auto act) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!there[k] || !on) continue;
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    const float2 xh = mul2(x[k][j], both(rstd)), n = fma2(xh, w[k][j], b[k][j]);
+                    float2 a, da;
+                    activate<T, act.value>(kGate ? g[k][j] : n, a, da);
+                    const float2 dn = mul2(d[k][j], kGate ? a : da);
+                    if (kGate) g[k][j] = mul2(mul2(d[k][j], n), da);
+                    dw[k][j] = fma2(dn, xh, dw[k][j]);
+                    db[k][j] = add2(db[k][j], dn);
+                    const float2 dxh = mul2(dn, w[k][j]);
+                    s1 = add2(s1, dxh);
+                    s2 = fma2(dxh, xh, s2);
+                    x[k][j] = xh;
+                    d[k][j] = dxh;
+                }
+            }
+        };
+        if (p.act == B200WKV_ACT_SILU) gradients(std::integral_constant<int, B200WKV_ACT_SILU>());
+        else if (p.act == B200WKV_ACT_SIGMOID) gradients(std::integral_constant<int, B200WKV_ACT_SIGMOID>());
+        else gradients(std::integral_constant<int, B200WKV_ACT_NONE>());
+        const float m1 = team_sum<kBlock>(sum_of<VEC>(s1), p.team, room) * inv_d, m2 = team_sum<kBlock>(sum_of<VEC>(s2), p.team, room) * inv_d;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (!there[k] || !on) continue;
+            if (kGate) store_piece<T, VEC>(dgate + dense + k * step, g[k]);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) d[k][j] = mul2(fma2(x[k][j], both(-m2), add2(d[k][j], both(-m1))), both(rstd));
+            store_piece<T, VEC>(dx + dense + k * step, d[k]);
         }
     }
     if (partial == nullptr) return;
     // partial rows (parallel or one per CTA, 2, C): weight, bias
+    const auto of = [](const float2* v, int i) { return i % 2 == 0 ? v[i / 2].x : v[i / 2].y; };
     if (!kBlock && p.reduce) {
         const int in_cta = threadIdx.x / p.team;
 #pragma unroll
@@ -276,29 +332,26 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
             for (int which = 0; which < 2; ++which) {
                 __syncthreads();
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) both[threadIdx.x * VEC + v] = which == 0 ? dw[k][v] : db[k][v];
+                for (int v = 0; v < VEC; ++v) both_sums[threadIdx.x * VEC + v] = of(which == 0 ? dw[k] : db[k], v);
                 __syncthreads();
-                if (in_cta < p.G && at.lane + k * p.team < pieces) {       // the first team of its group adds the others
+                if (in_cta < p.G && there[k])              // the first team of its group adds the others
                     for (int v = 0; v < VEC; ++v) {
                         float t = 0.f;
-                        for (int j = in_cta; j < p.per_cta; j += p.G) t += both[(j * p.team + at.lane) * VEC + v];
-                        partial[((size_t)blockIdx.x * 2 + which) * p.C + c0 + (at.lane + k * p.team) * VEC + v] = t;
+                        for (int j = in_cta; j < p.per_cta; j += p.G) t += both_sums[(j * p.team + at.lane) * VEC + v];
+                        partial[((size_t)blockIdx.x * 2 + which) * p.C + c + k * step + v] = t;
                     }
-                }
             }
         return;
     }
-    if (!at.at_work) return;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int piece = at.lane + k * p.team;
-        if (piece >= pieces) continue;
+    for (int k = 0; k < K; ++k)
+        if (there[k]) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            partial[((size_t)at.first * 2) * p.C + c0 + piece * VEC + v] = dw[k][v];
-            partial[((size_t)at.first * 2 + 1) * p.C + c0 + piece * VEC + v] = db[k][v];
+            for (int v = 0; v < VEC; ++v) {
+                partial[((size_t)at.first * 2) * p.C + c + k * step + v] = of(dw[k], v);
+                partial[((size_t)at.first * 2 + 1) * p.C + c + k * step + v] = of(db[k], v);
+            }
         }
-    }
 }
 
 // The partial rows' sums, in the parameters' type: a CTA owns 32 of the 2 C columns, its warps every sixteenth row, added in a fixed order.
@@ -409,7 +462,8 @@ int bwd(cudaStream_t st, Problem p, const void* gy, void* dx, void* dgate, void*
 Problem problem(long long rows, int C, int groups, float eps, int act, const void* x, long long x_stride, const void* weight, const void* bias,
                 int param_dtype, const void* gate, long long gate_stride) {
     const int f32 = param_dtype == B200WKV_F32;
-    return {rows, C, groups, C / groups, act, eps, x, gate, x_stride, gate != nullptr ? gate_stride : 0, {weight, f32}, {bias, f32}, 0, 0, 0, 0};
+    return {rows, C, groups, C / groups, act, eps, x, gate, x_stride, gate != nullptr ? gate_stride : 0, {weight, f32}, {bias, f32}, 0, 0, 0,
+            on_16({weight, bias}, {}, 4), 0};
 }
 }  // namespace
 

@@ -19,6 +19,8 @@
 // from the last to the first with the same products A.
 //
 // A start flag cuts by a select, not by a factor of 0: what is no number in front of it ends there.
+#include <limits.h>
+
 #include <initializer_list>
 
 #include "common.cuh"
@@ -479,26 +481,61 @@ gated_step_kernel(int B, int C, const T* x, long long x_stride, const T* f, long
     *(Few<float, V>*)(s_out + bi * s_out_stride + c) = rh;
 }
 
-// CTAs of a cluster: as many as it takes to have two on every SM, no more than there are tiles.
-int ranks_of(int units, int tiles) {
-    int n = 1;
-    while (n < kMaxCluster && n < tiles && units * n < 2 * sm_count_of_current_device()) n *= 2;
-    return n;
+// How many clusters of n CTAs a kernel has on the device at a time, asked once per device and kernel (which sets its shared memory too).
+struct Residency {
+    DeviceOnce once;
+    int clusters[kMaxDevices][kMaxCluster + 1];
+    template <typename Kernel> const int* of(Kernel kern, size_t smem) {
+        const int dev = current_device();
+        if (dev < 0) return nullptr;
+        const bool ok = once.ok([&]() {
+            const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            for (int n = 1; n <= kMaxCluster; ++n) {
+                cudaLaunchAttribute attr[1];
+                cudaLaunchConfig_t cfg = config(attr, n, n, smem, nullptr);
+                int fit = 0;
+                if (cudaOccupancyMaxActiveClusters(&fit, kern, &cfg) != cudaSuccess) {
+                    (void)cudaGetLastError();
+                    fit = 0;               // no cluster of this size
+                }
+                clusters[dev][n] = fit;
+            }
+            return e;
+        });
+        return ok ? clusters[dev] : nullptr;
+    }
+    static cudaLaunchConfig_t config(cudaLaunchAttribute* attr, int ranks, unsigned grid, size_t smem, cudaStream_t st) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(kWarps * 32);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return cfg;
+    }
+};
+// CTAs of a cluster: those with which the last sequence is done after the fewest rounds, waves of clusters counted; the smaller of equals.
+// units: 64 channels of a sequence each; tiles: of one of them.
+int ranks_of(const int* resident, long long units, int tiles) {
+    int best = 1;
+    long long least = LLONG_MAX;
+    for (int n = 1; n <= kMaxCluster && n <= tiles; ++n) {
+        if (resident[n] < 1) continue;
+        const long long rounds = (units + resident[n] - 1) / resident[n] * ((tiles + n - 1) / n);
+        if (rounds < least) { least = rounds; best = n; }
+    }
+    return best;
 }
 template <typename Kernel, typename... Args>
-int launch(DeviceOnce& once, Kernel kern, cudaStream_t st, int B, const Problem& p, int tile, size_t smem, Args... args) {
-    if (!once.ok([&]() { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); })) return B200WKV_ELAUNCH;
-    const int ranks = ranks_of(B * p.slabs, (p.T + tile - 1) / tile);
+int launch(Residency& residency, Kernel kern, cudaStream_t st, int B, const Problem& p, int tile, size_t smem, Args... args) {
+    const int* const resident = residency.of(kern, smem);
+    if (resident == nullptr) return B200WKV_ELAUNCH;
+    const int units = B * p.slabs, ranks = ranks_of(resident, units, (p.T + tile - 1) / tile);
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(B * p.slabs * ranks));
-    cfg.blockDim = dim3(kWarps * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    const cudaLaunchConfig_t cfg = Residency::config(attr, ranks, (unsigned)units * ranks, smem, st);
     return cudaLaunchKernelEx(&cfg, kern, p, args...) == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
 }
 // The widest pieces that every row of these begins on.
@@ -510,13 +547,13 @@ int piece_of(int C, int element, std::initializer_list<const void*> streams, std
 }
 
 template <typename T, int kGate, int kPiece> int fwd(cudaStream_t st, int B, const Problem& p, void* y, float* s_out, float* kept) {
-    static DeviceOnce once;
+    static Residency once;
     constexpr int kTile = kFwdSeg<T> * kWarps;
     return launch(once, gated_fwd_kernel<T, kGate, kPiece>, st, B, p, kTile, (size_t)kStages * 2 * kTile * kWide * sizeof(T), (T*)y, s_out, kept);
 }
 template <typename T, int kGate, int kPiece>
 int bwd(cudaStream_t st, int B, const Problem& p, const void* gy, const float* gs, const float* kept, void* dx, void* df, float* ds0) {
-    static DeviceOnce once;
+    static Residency once;
     return launch(once, gated_bwd_kernel<T, kGate, kPiece>, st, B, p, kKept, (size_t)kStages * 3 * kKept * kWide * sizeof(T), (const T*)gy, gs, kept,
                   (T*)dx, (T*)df, ds0);
 }

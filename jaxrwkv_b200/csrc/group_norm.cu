@@ -359,13 +359,13 @@ __global__ void __launch_bounds__(512) group_norm_sums_kernel(const float* parti
     __shared__ float part[16][32];
     wait_for_grid_in_front();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    float s[8] = {};
     if (c < 2 * C)
-        for (int r = warp; r < rows; r += 64)
+        for (int r = warp; r < rows; r += 128)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 8; ++j)
                 if (r + 16 * j < rows) s[j] += partial[(size_t)(r + 16 * j) * 2 * C + c];
-    part[warp][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+    part[warp][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (warp != 0 || c >= 2 * C) return;
     float t = 0.f;
@@ -447,7 +447,7 @@ template <typename T> int fwd(cudaStream_t st, Problem p, void* y) {
 }
 template <typename T>
 int bwd(cudaStream_t st, Problem p, const void* gy, void* dx, void* dgate, void* dweight, void* dbias, float* partial) {
-    const Plan q = plan_of(p, sizeof(T), on_16({p.x, p.gate, gy, dx, dgate}, {p.x_stride, p.gate_stride}, sizeof(T)), 4);
+    const Plan q = plan_of(p, sizeof(T), on_16({p.x, p.gate, gy, dx, dgate}, {p.x_stride, p.gate_stride}, sizeof(T)), 2);
     const bool params = dweight != nullptr || dbias != nullptr;
     if (!params) partial = nullptr;
     const int status = dispatch<T>(q, p, [&](auto vec, auto k, auto block, auto gate) {

@@ -552,11 +552,11 @@ int b200wkv_token_shift_bwd(void* stream, int dtype, int B, int T, int D, int M,
 static bool known(int dtype) { return dtype == B200WKV_F32 || dtype == B200WKV_BF16; }
 static size_t element_bytes(int dtype) { return dtype == B200WKV_F32 ? 4 : 2; }
 
-// The tiles of a sequence are counted and the grid is made in 32 bits.
+// The tiles of a sequence are counted and the grid is made in 32 bits, and so are offsets inside a tile of 128 tokens.
 static int check_gated(int dtype, int gate, int B, int T, int C) {
     if (!known(dtype)) return B200WKV_EDTYPE;
     if (gate != B200WKV_GATE_SIGMOID && gate != B200WKV_GATE_DECAY) return B200WKV_EUNSUPPORTED;
-    if (B < 1 || T < 1 || C < 1 || (long long)B * T > 2147483647LL || T > (1 << 30) || (long long)B * C > (1LL << 30)) return B200WKV_ESHAPE;
+    if (B < 1 || T < 1 || C < 1 || (long long)B * T > 2147483647LL || T > (1 << 30) || C > (1 << 22) || (long long)B * C > (1LL << 30)) return B200WKV_ESHAPE;
     return B200WKV_OK;
 }
 

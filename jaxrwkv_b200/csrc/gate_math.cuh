@@ -22,43 +22,52 @@ __device__ __forceinline__ float min_nan(float x, float y) {
     return r;
 }
 
-// Two numbers in one instruction: these kernels are short of issue slots before anything else.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+// Two numbers in one instruction: these kernels are short of issue slots before anything else.  They stay in one 64-bit register
+// from instruction to instruction; as two 32-bit values they would be moved together and apart around each.
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 make_f2(float x, float y) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
     return r;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+__device__ __forceinline__ float2 parts(F2 a) {
     float2 r;
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
     return r;
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return r;
 }
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 both(float x) { return make_f2(x, x); }
 // two adjacent elements
-__device__ __forceinline__ float2 unpack_pair(uint32_t q) { return make_float2(__uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u)); }
+__device__ __forceinline__ F2 unpack_pair(uint32_t q) { return make_f2(__uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u)); }
 
 // p = sigmoid(z) and q = 1 - p = p e^-z, both to full relative precision.  The exponential is kept below 2^126, so that neither factor
 // leaves the range (p is at least 2^-126 then, and not 0).  For bf16 streams by the hardware's exponential, whose argument's
 // rounding is 2^-24 |z| at most.
-template <typename T> __device__ __forceinline__ void sigmoid_pair(float2 z, float2& p, float2& q) {
-    float2 e;
+template <typename T> __device__ __forceinline__ void sigmoid_pair(F2 z, F2& p, F2& q) {
+    F2 e;
     if constexpr (sizeof(T) == 4) {
-        e = make_float2(expf(min_nan(-z.x, 87.f)), expf(min_nan(-z.y, 87.f)));
+        const float2 t = parts(z);
+        e = make_f2(expf(min_nan(-t.x, 87.f)), expf(min_nan(-t.y, 87.f)));
     } else {
-        const float2 t = mul2(z, both(-1.44269504f));
-        e = make_float2(ex2_approx(min_nan(t.x, 126.f)), ex2_approx(min_nan(t.y, 126.f)));
+        const float2 t = parts(mul2(z, both(-1.44269504f)));
+        e = make_f2(ex2_approx(min_nan(t.x, 126.f)), ex2_approx(min_nan(t.y, 126.f)));
     }
-    const float2 d = add2(e, both(1.f));
-    p = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    const float2 d = parts(add2(e, both(1.f)));
+    p = make_f2(rcp_approx(d.x), rcp_approx(d.y));
     q = mul2(e, p);
 }
 

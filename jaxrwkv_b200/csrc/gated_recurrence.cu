@@ -42,22 +42,25 @@ constexpr int kStages = 2;
 constexpr int kWaitRanOut = 3;             // status word: a wait for the other CTAs of a cluster
 
 // two channels, as they lie in shared memory
-__device__ __forceinline__ float2 pair_at(const float* p) { return *reinterpret_cast<const float2*>(p); }
-__device__ __forceinline__ float2 pair_at(const __nv_bfloat16* p) { return unpack_pair(*reinterpret_cast<const uint32_t*>(p)); }
-__device__ __forceinline__ void store_pair(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
-__device__ __forceinline__ void store_pair(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
+__device__ __forceinline__ F2 pair_at(const float* p) { return *reinterpret_cast<const F2*>(p); }
+__device__ __forceinline__ F2 pair_at(const __nv_bfloat16* p) { return unpack_pair(*reinterpret_cast<const uint32_t*>(p)); }
+__device__ __forceinline__ void store_pair(float* p, F2 a) { *reinterpret_cast<F2*>(p) = a; }
+__device__ __forceinline__ void store_pair(__nv_bfloat16* p, F2 a) {
+    const float2 q = parts(a);
+    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(q.x, q.y);
+}
 
 constexpr int kSigmoidGate = B200WKV_GATE_SIGMOID;
 // The gate a, and what the backward needs of it: `w`, for the sigmoid 1 - a (to full relative precision), for the decay -da/df.
-template <typename T, int kGate> __device__ __forceinline__ void gate_of(float2 f, float2& a, float2& w) {
+template <typename T, int kGate> __device__ __forceinline__ void gate_of(F2 f, F2& a, F2& w) {
     if (kGate == kSigmoidGate) {
         sigmoid_pair<T>(f, a, w);
     } else {
         // (accurate in 16 bits too: the state sums 1 / (1 - a) tokens, and an error of a is that much larger in it)
-        const float2 e = make_float2(expf(f.x), expf(f.y));
-        a = make_float2(expf(-e.x), expf(-e.y));
-        w = mul2(e, a);
-        w = make_float2(a.x == 0.f ? 0.f : w.x, a.y == 0.f ? 0.f : w.y);        // (e may be infinite then)
+        const float2 z = parts(f);
+        const float e0 = expf(z.x), e1 = expf(z.y), a0 = expf(-e0), a1 = expf(-e1);
+        a = make_f2(a0, a1);
+        w = make_f2(a0 == 0.f ? 0.f : e0 * a0, a1 == 0.f ? 0.f : e1 * a1);      // (e may be infinite then)
     }
 }
 
@@ -66,7 +69,7 @@ struct Stream {                            // rows of C adjacent channels
     long long batch, token;                // strides in elements
 };
 struct Problem {
-    int T, C, slabs;
+    int B, T, C;
     Stream x, f;
     const float* s0;
     const uint32_t* length;
@@ -74,55 +77,63 @@ struct Problem {
     int* status;
 };
 
-// What a stretch does to the state of a channel: h -> A h + b.  A's sign bit says that a start flag lies inside: h is dropped.
-__device__ __forceinline__ bool cuts(float A) { return __float_as_int(A) < 0; }
-__device__ __forceinline__ float behind(float A, float b, float h) { return cuts(A) ? b : fmaf(A, h, b); }
-struct Stretch {
-    float4 v;                              // A, b of the lane's first channel, then of its second
-    __device__ __forceinline__ static Stretch nothing() { return {make_float4(1.f, 0.f, 1.f, 0.f)}; }
-    __device__ __forceinline__ void follow(float4 n) {               // by the stretch n
-        v.y = behind(n.x, n.y, v.y);
-        v.w = behind(n.z, n.w, v.w);
-        v.x = cuts(n.x) ? -1.f : v.x * n.x;
-        v.z = cuts(n.z) ? -1.f : v.z * n.z;
-    }
-    __device__ __forceinline__ float2 of(float2 h) const { return make_float2(behind(v.x, v.y, h.x), behind(v.z, v.w, h.y)); }
+// What a stretch does to the states of two channels: h -> A h + b.  A start flag inside, which drops h, makes both A negative (-0 is).
+// Either says it for both: a gate that is no number takes the sign of its channel, whose b is no number then either.
+__device__ __forceinline__ bool negative(float A) { return __float_as_uint(A) + 0x80000000u <= 0x7f800000u; }
+__device__ __forceinline__ bool cuts(F2 A) {
+    const float2 q = parts(A);
+    return negative(q.x) || negative(q.y);
+}
+struct alignas(16) Stretch {
+    F2 A, b;
+    __device__ __forceinline__ static Stretch nothing() { return {both(1.f), both(0.f)}; }
+    __device__ __forceinline__ F2 of_uncut(F2 h) const { return fma2(A, h, b); }
+    __device__ __forceinline__ F2 of(F2 h) const { return cuts(A) ? b : fma2(A, h, b); }
+    __device__ __forceinline__ Stretch then(const Stretch& n) const { return {cuts(n.A) ? both(-1.f) : mul2(A, n.A), n.of(b)}; }
 };
 
-// A warp's segments of one stream on their way to shared memory: kSeg rows of 64 channels, zeros behind the sequence's end and the
-// last channel.  Pieces of kPiece bytes; 2: single 16-bit elements, which no asynchronous copy takes.
+// A CTA's tiles of one stream on their way to shared memory, each warp its segment: kSeg rows of 64 channels, zeros behind the sequence's
+// end and the last channel.  Pieces of kPiece bytes; 2: single 16-bit elements, which no asynchronous copy takes.  Addresses are a
+// base that is the same for the CTA and 32 bits of the lane's own, where a tile of whole rows is that near.
 template <typename T, int kPiece, int kSeg> struct Feed {
     static constexpr int kPer = kPiece / (int)sizeof(T), kPerRow = kWide / kPer;
     static constexpr int kRows = kPerRow <= 32 ? 32 / kPerRow : 1, kPasses = kPerRow <= 32 ? 1 : kPerRow / 32;
-    const T* from;                         // the lane's first piece of token 0
-    long long stride;
-    int row, c, left;                      // the lane's first row and channel; channels that there are
-    __device__ __forceinline__ Feed(const void* p, long long batch, long long token, int bi, int c0, int C, int lane)
-        : stride(token), row(kPasses == 1 ? lane / kPerRow : 0), c((kPasses == 1 ? lane % kPerRow : lane) * kPer), left(C - c0) {
-        from = (const T*)p + bi * batch + c0;
+    const char* base;                      // token 0 of the CTA's channels
+    long long stride;                      // bytes from token to token
+    uint32_t off;                          // the lane's first piece in a tile
+    int left;                              // channels that there are
+    bool near;
+    __device__ __forceinline__ static int row() { return kPasses == 1 ? (int)(threadIdx.x & 31) / kPerRow : 0; }
+    __device__ __forceinline__ static int channel() { return (int)(kPasses == 1 ? (threadIdx.x & 31) % kPerRow : threadIdx.x & 31) * kPer; }
+    __device__ __forceinline__ Feed(const void* p, long long batch, long long token, int bi, int c0, int C)
+        : base((const char*)p + (bi * batch + c0) * (long long)sizeof(T)), stride(token * (long long)sizeof(T)), left(C - c0) {
+        near = stride * (kSeg * kWarps) < (1LL << 31) && left >= kWide;
+        off = (uint32_t)((threadIdx.x / 32 * kSeg + row()) * (uint32_t)stride + channel() * sizeof(T));
     }
-    __device__ __forceinline__ static void piece(T* to, const T* from, bool valid) {
-        if constexpr (kPiece == 16) cp_async16(to, from, valid);
-        else if constexpr (kPiece == 4)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(valid ? 4 : 0) : "memory");
-        else *to = valid ? *from : from_f32<T>(0.f);
+    __device__ __forceinline__ static void piece(uint32_t to, const char* from, bool valid) {
+        if constexpr (kPiece == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+        else if constexpr (kPiece == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(valid ? 4 : 0) : "memory");
+        else asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(valid ? *(const unsigned short*)from : (unsigned short)0) : "memory");
     }
-    __device__ __forceinline__ void fetch(T* to, int t0, int Tlen) const {
-        to += row * kWide + c;
-        if (t0 + kSeg <= Tlen && left >= kWide) {
-            const T* at = from + (t0 + row) * stride + c;
+    // the tile that begins at t0; `to`: the warp's rows in shared memory
+    __device__ __forceinline__ void fetch(uint32_t to, int t0, int Tlen) const {
+        to += (row() * kWide + channel()) * sizeof(T);
+        if (near && t0 + kSeg * kWarps <= Tlen) {
+            const char* const tile = base + t0 * stride;
+            const uint32_t down = (uint32_t)(kRows * stride);
+            uint32_t at = off;
 #pragma unroll
-            for (int i = 0; i < kSeg; i += kRows, at += kRows * stride)
+            for (int i = 0; i < kSeg; i += kRows, at += down)
 #pragma unroll
-                for (int pass = 0; pass < kPasses; ++pass) piece(to + i * kWide + pass * 32 * kPer, at + pass * 32 * kPer, true);
+                for (int pass = 0; pass < kPasses; ++pass) piece(to + (i * kWide + pass * 32 * kPer) * sizeof(T), tile + at + pass * 32 * kPiece, true);
         } else {
-#pragma unroll
+            const int first = t0 + (int)(threadIdx.x / 32) * kSeg + row();
             for (int i = 0; i < kSeg; i += kRows)
 #pragma unroll
                 for (int pass = 0; pass < kPasses; ++pass) {
-                    const int t = t0 + i + row, ch = c + pass * 32 * kPer;
-                    const bool valid = t < Tlen && ch < left;
-                    piece(to + i * kWide + pass * 32 * kPer, from + (valid ? t * stride + ch : 0), valid);
+                    const int c = channel() + pass * 32 * kPer;
+                    const bool valid = first + i < Tlen && c < left;
+                    piece(to + (i * kWide + pass * 32 * kPer) * sizeof(T), base + (valid ? (first + i) * stride + c * (long long)sizeof(T) : 0), valid);
                 }
         }
     }
@@ -133,21 +144,22 @@ template <int kLeft> __device__ __forceinline__ void wait_fetched() {
     __syncwarp();
 }
 
-// A pair of channels of a dense row; single elements where pairs do not fit the row (kPiece one element) or its end
-template <typename T, int kPiece> __device__ __forceinline__ void put(T* p, float a, float b, int channels) {
+// A pair of channels of a dense row; single elements where pairs do not fit the row (kPiece one element), whose last may have no second.
+// (A lane behind the last channel goes along with the last pair, and writes what that writes.)
+template <typename T, int kPiece> __device__ __forceinline__ void put(T* p, F2 a, int channels) {
     if constexpr (kPiece >= 2 * (int)sizeof(T)) {
-        if (channels > 0) store_pair(p, a, b);
+        store_pair(p, a);
     } else {
-        if (channels > 0) p[0] = from_f32<T>(a);
-        if (channels > 1) p[1] = from_f32<T>(b);
+        const float2 q = parts(a);
+        p[0] = from_f32<T>(q.x);
+        if (channels > 1) p[1] = from_f32<T>(q.y);
     }
 }
-__device__ __forceinline__ float2 get_state(const float* p, int channels) {
-    return make_float2(p != nullptr && channels > 0 ? p[0] : 0.f, p != nullptr && channels > 1 ? p[1] : 0.f);
-}
-__device__ __forceinline__ void put_state(float* p, float2 h, int channels) {
-    if (channels > 0) p[0] = h.x;
-    if (channels > 1) p[1] = h.y;
+__device__ __forceinline__ F2 get_state(const float* p, int channels) { return make_f2(p != nullptr ? p[0] : 0.f, p != nullptr && channels > 1 ? p[1] : 0.f); }
+__device__ __forceinline__ void put_state(float* p, F2 h, int channels) {
+    const float2 q = parts(h);
+    p[0] = q.x;
+    if (channels > 1) p[1] = q.y;
 }
 
 // start flags of the kSeg tokens from t0 on as a bit mask (bit i = token t0 + i)
@@ -159,7 +171,7 @@ template <int kSeg> __device__ __forceinline__ uint32_t segment_flags(const uint
 // What the CTAs of a cluster tell one another: the stretches of a round's tiles.  Two rounds' worth: a CTA sends a round's only when
 // it has those of the round in front from everyone, who by then have used the round before that.
 struct Exchange {
-    float4 tiles[2][kMaxCluster][32];
+    Stretch tiles[2][kMaxCluster][32];
     uint64_t bar[2];
     __device__ __forceinline__ void open(int ranks) {
         if (threadIdx.x == 0) {
@@ -171,8 +183,9 @@ struct Exchange {
     }
     __device__ __forceinline__ void send(int round, int rank, int ranks, const Stretch& tile, int lane) {   // by one warp
         uint64_t* const mine = &bar[round & 1];
-        if (lane == 0) mbar_expect_tx(mine, (uint32_t)ranks * 32 * sizeof(float4));
-        for (int q = 0; q < ranks; ++q) store_in_cta(in_cta(&tiles[round & 1][rank][lane], q), tile.v, in_cta(mine, q));
+        if (lane == 0) mbar_expect_tx(mine, (uint32_t)ranks * 32 * sizeof(Stretch));
+        const float2 A = parts(tile.A), b = parts(tile.b);
+        for (int q = 0; q < ranks; ++q) store_in_cta(in_cta(&tiles[round & 1][rank][lane], q), make_float4(A.x, A.y, b.x, b.y), in_cta(mine, q));
     }
     __device__ __forceinline__ void wait(int round, bool& lost, int* status) {
         if (lost || mbar_wait_cluster(&bar[round & 1], (round >> 1) & 1)) return;
@@ -183,22 +196,52 @@ struct Exchange {
     __device__ __forceinline__ void close(int ranks) { if (ranks > 1) cluster_sync(); }
 };
 
+// Grid: x the 64 channels and, inside, the CTAs of a cluster; y and z the sequence
 struct Place {
-    int rank, ranks, lane, warp, bi, c, channels, L;
-    size_t state;                          // the lane's first channel in a dense (B, C) array
+    int rank, ranks, lane, warp, bi, c0, col, channels, L;
     __device__ __forceinline__ Place(const Problem& p) {
         rank = (int)cluster_rank(); ranks = (int)cluster_size();
-        lane = threadIdx.x & 31; warp = threadIdx.x >> 5;
-        const int unit = blockIdx.x / ranks;
-        bi = unit / p.slabs;
-        c = unit % p.slabs * kWide + 2 * lane;
-        channels = p.C - c;
-        L = p.length != nullptr ? (int)min(p.length[bi], (uint32_t)p.T) : p.T;
-        state = (size_t)bi * p.C + c;
+        lane = threadIdx.x & 31;
+        warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+        bi = blockIdx.y + blockIdx.z * gridDim.y;
+        unsigned slab;
+        asm("mov.u32 %0, %%clusterid.x;" : "=r"(slab));
+        c0 = (int)slab * kWide;
+        col = min(2 * lane, (p.C - c0 - 1) & ~1);
+        channels = p.C - c0 - col;
+        L = p.length != nullptr && bi < p.B ? (int)min(p.length[bi], (uint32_t)p.T) : p.T;
     }
+    __device__ __forceinline__ size_t state(const Problem& p) const { return (size_t)bi * p.C + c0 + col; }      // in a dense (B, C) array
 };
 struct Plain { static constexpr bool value = true; };      // a whole segment without a start flag in which the returned state is not taken
 struct Marked { static constexpr bool value = false; };
+
+// The segments of a tile by what they do to a state, in the order in which it meets them, behind as many identities as there are
+// segments in front of the last one: every warp goes over seven.
+struct Chain {
+    Stretch s[kWarps - 1 + kWarps][32];
+    __device__ __forceinline__ void pad() {
+        for (int i = threadIdx.x; i < (kWarps - 1) * 32; i += kWarps * 32) s[i / 32][i % 32] = Stretch::nothing();
+    }
+    __device__ __forceinline__ Stretch& of(int place) { return s[kWarps - 1 + place][threadIdx.x & 31]; }
+    // the state that enters the first segment, as it enters the one at `place`
+    __device__ __forceinline__ F2 follow(F2 h, int place, bool marked) const {
+        const Stretch(*const q)[32] = &s[place];
+        if (!marked) {
+#pragma unroll
+            for (int j = 0; j < kWarps - 1; ++j) h = q[j][threadIdx.x & 31].of_uncut(h);
+        } else {
+            for (int j = 0; j < kWarps - 1; ++j) h = q[j][threadIdx.x & 31].of(h);
+        }
+        return h;
+    }
+    __device__ __forceinline__ Stretch all() {
+        Stretch t = of(0);
+#pragma unroll
+        for (int j = 1; j < kWarps; ++j) t = t.then(of(j));
+        return t;
+    }
+};
 
 template <typename T> constexpr int kFwdSeg = sizeof(T) == 2 ? 16 : 8;
 constexpr int kBwdSeg = kKept / kWarps;
@@ -206,51 +249,54 @@ constexpr int kBwdSeg = kKept / kWarps;
 template <typename T, int kGate, int kPiece>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, float* __restrict__ kept) {
-    constexpr int kSeg = kFwdSeg<T>, kTile = kSeg * kWarps, kHalf = kSeg * kWide;
+    constexpr int kSeg = kFwdSeg<T>, kTile = kSeg * kWarps, kRow = kWide * (int)sizeof(T), kRoom = 2 * kSeg * kRow;
     extern __shared__ __align__(128) unsigned char dynamic[];
     __shared__ Exchange ex;
-    __shared__ float4 segs[2][kWarps][32];
-    __shared__ float2 carried[2][32];
+    __shared__ Chain chain[2];
+    __shared__ F2 carried[2][32];
     const Place at(p);
-    const int lane = at.lane, warp = at.warp, ranks = at.ranks, tiles = (p.T + kTile - 1) / kTile, rounds = (tiles + ranks - 1) / ranks;
-    const Feed<T, kPiece, kSeg> fx(p.x.p, p.x.batch, p.x.token, at.bi, at.c - 2 * lane, p.C, lane);
-    const Feed<T, kPiece, kSeg> ff(p.f.p, p.f.batch, p.f.token, at.bi, at.c - 2 * lane, p.C, lane);
-    T* const room = (T*)dynamic + warp * kStages * 2 * kHalf;
-    const auto first = [&](int round) { return (round * ranks + at.rank) * kTile + warp * kSeg; };
+    if (at.bi >= p.B) return;              // (a whole cluster)
+    const int lane = at.lane, warp = at.warp, ranks = at.ranks, c0 = at.c0;
+    const size_t state = at.state(p);
+    const int tiles = (p.T + kTile - 1) / kTile, rounds = (tiles + ranks - 1) / ranks;
+    const Feed<T, kPiece, kSeg> fx(p.x.p, p.x.batch, p.x.token, at.bi, c0, p.C), ff(p.f.p, p.f.batch, p.f.token, at.bi, c0, p.C);
+    unsigned char* const room = dynamic + warp * kStages * kRoom;
     const auto ask = [&](int round) {
         if (round < rounds) {
-            T* const to = room + round % kStages * 2 * kHalf;
-            fx.fetch(to, first(round), p.T);
-            ff.fetch(to + kHalf, first(round), p.T);
+            const uint32_t to = smem_u32(room) + round % kStages * kRoom;
+            fx.fetch(to, (round * ranks + at.rank) * kTile, p.T);
+            ff.fetch(to + kSeg * kRow, (round * ranks + at.rank) * kTile, p.T);
         }
         fetched();
     };
     for (int i = 0; i < kStages; ++i) ask(i);
-    float2 carry = get_state(p.s0 != nullptr ? p.s0 + at.state : nullptr, at.channels);      // state entering the round
-    if (at.L == 0 && warp == 0 && at.rank == 0) put_state(s_out + at.state, carry, at.channels);
+    F2 carry = get_state(p.s0 != nullptr ? p.s0 + state : nullptr, at.channels);      // state entering the round
+    if (at.L == 0 && warp == 0 && at.rank == 0) put_state(s_out + state, carry, at.channels);
     if (warp == kWarps - 1) carried[0][lane] = carry;
+    chain[0].pad();
+    chain[1].pad();
     ex.open(ranks);
     bool lost = false;
-    T* const py = y + (size_t)at.bi * p.T * p.C + at.c;
     const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)at.bi * p.T : nullptr;
+    const uint32_t down = p.C * (uint32_t)sizeof(T), own_off = warp * kSeg * down + at.col * (uint32_t)sizeof(T);
     for (int round = 0; round < rounds; ++round) {
-        const int t0 = first(round), n = max(0, min(kSeg, p.T - t0)), parity = round & 1;
+        const int tile = (round * ranks + at.rank) * kTile, t0 = tile + warp * kSeg, n = max(0, min(kSeg, p.T - t0)), parity = round & 1;
         const uint32_t starts = segment_flags<kSeg>(ns, t0, p.T, lane);
         const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
         // 1. gates and increments, and what the segment does
-        float2 a[kSeg], u[kSeg];
+        F2 a[kSeg], u[kSeg];
         wait_fetched<kStages - 1>();
-        const T* const from = room + round % kStages * 2 * kHalf + 2 * lane;
+        const T* const from = (const T*)(room + round % kStages * kRoom) + at.col;
 #pragma unroll
         for (int i = 0; i < kSeg; ++i) {
-            const float2 x = pair_at(from + i * kWide);
-            float2 w;
-            gate_of<T, kGate>(pair_at(from + kHalf + i * kWide), a[i], w);
+            const F2 x = pair_at(from + i * kWide);
+            F2 w;
+            gate_of<T, kGate>(pair_at(from + (kSeg + i) * kWide), a[i], w);
             u[i] = kGate == kSigmoidGate ? mul2(w, x) : x;
         }
         __syncwarp();                      // the segment has been read
         ask(round + kStages);
-        float2 A = both(1.f), b = both(0.f);
+        F2 A = both(1.f), b = both(0.f);
         const auto summarise = [&](auto kind) {
 #pragma unroll
             for (int i = 0; i < kSeg; ++i) {
@@ -263,45 +309,33 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
             }
         };
         if (plain) summarise(Plain()); else summarise(Marked());
-        const Stretch own = {make_float4(A.x, b.x, A.y, b.y)};
-        segs[parity][warp][lane] = own.v;
-        __syncthreads();
-        // 2. the state that enters the segment
-        float2 h;
+        chain[parity].of(warp) = Stretch{A, b};
+        const bool marked = __syncthreads_or(starts != 0);       // a start flag in the tile
+        // 2. the state that enters the tile, and the one that enters the segment
+        F2 h;
         if (ranks > 1) {
-            Stretch front = Stretch::nothing();
-#pragma unroll
-            for (int j = 0; j < kWarps - 1; ++j)
-                if (j < warp) front.follow(segs[parity][j][lane]);
-            if (warp == kWarps - 1) {
-                Stretch tile = front;
-                tile.follow(own.v);
-                ex.send(round, at.rank, ranks, tile, lane);
-            }
+            if (warp == kWarps - 1) ex.send(round, at.rank, ranks, chain[parity].all(), lane);
             ex.wait(round, lost, p.status);
             for (int q = 0; q < ranks; ++q) {
                 if (q == at.rank) h = carry;
-                const Stretch tile = {ex.tiles[parity][q][lane]};
-                carry = tile.of(carry);
+                carry = ex.tiles[parity][q][lane].of(carry);
             }
-            h = front.of(h);
         } else {
             h = carried[parity][lane];
-#pragma unroll
-            for (int j = 0; j < kWarps - 1; ++j)
-                if (j < warp) h = Stretch{segs[parity][j][lane]}.of(h);
         }
+        h = chain[parity].follow(h, warp, marked);
         // (a kept state is wanted in front of every 64th token; the returned one behind its token)
-        if (kept != nullptr && n > 0 && t0 % kKept == 0) put_state(kept + ((size_t)at.bi * ((p.T + kKept - 1) / kKept) + t0 / kKept) * p.C + at.c, h, at.channels);
+        if (kept != nullptr && n > 0 && t0 % kKept == 0) put_state(kept + ((size_t)at.bi * ((p.T + kKept - 1) / kKept) + t0 / kKept) * p.C + c0 + at.col, h, at.channels);
         // 3. outputs
-        T* to = py + (size_t)t0 * p.C;
+        char* const to = (char*)y + (((long long)at.bi * p.T + tile) * p.C + c0) * (long long)sizeof(T);
         const auto walk = [&](auto kind) {
+            uint32_t off = own_off;
 #pragma unroll
-            for (int i = 0; i < kSeg; ++i, to += p.C) {
+            for (int i = 0; i < kSeg; ++i, off += down) {
                 const bool start = !kind.value && ((starts >> i) & 1u);
                 h = start ? u[i] : fma2(a[i], h, u[i]);
-                if (kind.value || i < n) put<T, kPiece>(to, h.x, h.y, at.channels);
-                if (!kind.value && t0 + i == at.L - 1) put_state(s_out + at.state, h, at.channels);
+                if (kind.value || i < n) put<T, kPiece>((T*)(to + off), h, at.channels);
+                if (!kind.value && t0 + i == at.L - 1) put_state(s_out + state, h, at.channels);
             }
         };
         if (plain) walk(Plain()); else walk(Marked());
@@ -314,60 +348,70 @@ template <typename T, int kGate, int kPiece>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restrict__ gs, const float* __restrict__ kept,
                  T* __restrict__ dx, T* __restrict__ df, float* __restrict__ ds0) {
-    constexpr int kSeg = kBwdSeg, kTile = kKept, kHalf = kSeg * kWide;
+    constexpr int kSeg = kBwdSeg, kTile = kKept, kRow = kWide * (int)sizeof(T), kRoom = 3 * kSeg * kRow;
     extern __shared__ __align__(128) unsigned char dynamic[];
     __shared__ Exchange ex;
-    __shared__ float4 segs[2][kWarps][32];
-    __shared__ float2 sent[2][kWarps][32], carried[2][32];
+    __shared__ Chain chain[2], back[2];
+    __shared__ F2 carried[2][32];
     const Place at(p);
-    const int lane = at.lane, warp = at.warp, ranks = at.ranks, tiles = (p.T + kTile - 1) / kTile, rounds = (tiles + ranks - 1) / ranks;
-    const Feed<T, kPiece, kSeg> fx(p.x.p, p.x.batch, p.x.token, at.bi, at.c - 2 * lane, p.C, lane);
-    const Feed<T, kPiece, kSeg> ff(p.f.p, p.f.batch, p.f.token, at.bi, at.c - 2 * lane, p.C, lane);
-    const Feed<T, kPiece, kSeg> fg(gy, (long long)p.T * p.C, p.C, at.bi, at.c - 2 * lane, p.C, lane);
-    T* const room = (T*)dynamic + warp * kStages * 3 * kHalf;
-    // rounds are taken from the last to the first; `done` of them lie behind
-    const auto first = [&](int done) { return ((rounds - 1 - done) * ranks + at.rank) * kTile + warp * kSeg; };
-    const auto ask = [&](int done) {
-        if (done < rounds) {
-            T* const to = room + done % kStages * 3 * kHalf;
-            fx.fetch(to, first(done), p.T);
-            ff.fetch(to + kHalf, first(done), p.T);
-            if (gy != nullptr) fg.fetch(to + 2 * kHalf, first(done), p.T);
+    if (at.bi >= p.B) return;              // (a whole cluster)
+    const int lane = at.lane, warp = at.warp, ranks = at.ranks, c0 = at.c0;
+    const size_t state = at.state(p);
+    const int tiles = (p.T + kTile - 1) / kTile, rounds = (tiles + ranks - 1) / ranks;
+    const Feed<T, kPiece, kSeg> fx(p.x.p, p.x.batch, p.x.token, at.bi, c0, p.C), ff(p.f.p, p.f.batch, p.f.token, at.bi, c0, p.C);
+    const Feed<T, kPiece, kSeg> fg(gy, (long long)p.T * p.C, p.C, at.bi, c0, p.C);
+    unsigned char* const room = dynamic + warp * kStages * kRoom;
+    // rounds are taken from the last to the first
+    const auto stage = [&](int round) { return (rounds - 1 - round) % kStages * kRoom; };
+    const auto ask = [&](int round) {
+        if (round >= 0) {
+            const uint32_t to = smem_u32(room) + stage(round);
+            const int tile = (round * ranks + at.rank) * kTile;
+            fx.fetch(to, tile, p.T);
+            ff.fetch(to + kSeg * kRow, tile, p.T);
+            if (gy != nullptr) fg.fetch(to + 2 * kSeg * kRow, tile, p.T);
         }
         fetched();
     };
-    const auto entering = [&](int done) {  // the kept state in front of a round's tile
-        const int tile = (rounds - 1 - done) * ranks + at.rank;
-        return done < rounds && tile < tiles ? get_state(kept + ((size_t)at.bi * tiles + tile) * p.C + at.c, at.channels) : make_float2(0.f, 0.f);
+    const auto entering = [&](int round) { // the kept state in front of a round's tile
+        const int tile = round * ranks + at.rank;
+        return round >= 0 && tile < tiles ? get_state(kept + ((long long)at.bi * tiles + tile) * p.C + c0 + at.col, at.channels) : both(0.f);
     };
-    for (int i = 0; i < kStages; ++i) ask(i);
-    float2 next = entering(0), carry = make_float2(0.f, 0.f);      // carry: c entering the round from behind
-    const float2 gstate = get_state(gs != nullptr ? gs + at.state : nullptr, at.channels);
-    if (warp == 0) carried[0][lane] = carry;
+    if (gy == nullptr)                     // nothing is fetched there, and zeros are read
+        for (int i = 0; i < kStages; ++i)
+            for (int j = lane; j < kSeg * kRow / 4; j += 32) ((uint32_t*)(room + i * kRoom + 2 * kSeg * kRow))[j] = 0;
+    for (int i = 0; i < kStages; ++i) ask(rounds - 1 - i);
+    F2 next = entering(rounds - 1), carry = both(0.f);       // carry: c entering the round from behind
+    const F2 gstate = get_state(gs != nullptr ? gs + state : nullptr, at.channels);
+    if (warp == 0) carried[(rounds - 1) & 1][lane] = carry;
+    chain[0].pad();
+    chain[1].pad();
+    back[0].pad();
+    back[1].pad();
     ex.open(ranks);
     bool lost = false;
-    const size_t base = (size_t)at.bi * p.T * p.C + at.c;
     const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)at.bi * p.T : nullptr;
-    for (int done = 0; done < rounds; ++done) {
-        const int t0 = first(done), n = max(0, min(kSeg, p.T - t0)), parity = done & 1;
+    const uint32_t down = p.C * (uint32_t)sizeof(T), own_off = (warp * kSeg + kSeg - 1) * down + at.col * (uint32_t)sizeof(T);
+    for (int round = rounds - 1; round >= 0; --round) {
+        const int tile = (round * ranks + at.rank) * kTile, t0 = tile + warp * kSeg, n = max(0, min(kSeg, p.T - t0)), parity = round & 1;
         const uint32_t starts = segment_flags<kSeg>(ns, t0, p.T, lane);
         const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
-        float2 h = next;
-        next = entering(done + 1);
+        F2 h = next;
+        next = entering(round - 1);
         // 1. gates; what the segment does to the states, and what it sends to the front
-        float2 a[kSeg], w[kSeg], x[kSeg], g[kSeg];
+        F2 a[kSeg], w[kSeg], x[kSeg], g[kSeg];
         wait_fetched<kStages - 1>();
-        const T* const from = room + done % kStages * 3 * kHalf + 2 * lane;
+        const T* const from = (const T*)(room + stage(round)) + at.col;
 #pragma unroll
         for (int i = 0; i < kSeg; ++i) {
             x[i] = pair_at(from + i * kWide);
-            gate_of<T, kGate>(pair_at(from + kHalf + i * kWide), a[i], w[i]);
-            g[i] = gy != nullptr ? pair_at(from + 2 * kHalf + i * kWide) : both(0.f);
+            gate_of<T, kGate>(pair_at(from + (kSeg + i) * kWide), a[i], w[i]);
+            g[i] = pair_at(from + (2 * kSeg + i) * kWide);
         }
         __syncwarp();                      // the segment has been read
-        ask(done + kStages);
+        ask(round - kStages);
         const auto increment = [&](int i) { return kGate == kSigmoidGate ? mul2(w[i], x[i]) : x[i]; };
-        float2 A = both(1.f), b = both(0.f), c = both(0.f);
+        F2 A = both(1.f), b = both(0.f), c = both(0.f);
         const auto summarise = [&](auto kind) {
 #pragma unroll
             for (int i = 0; i < kSeg; ++i) {
@@ -383,67 +427,48 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
             for (int i = kSeg - 1; i >= 0; --i) c = !kind.value && ((starts >> i) & 1u) ? both(0.f) : mul2(a[i], add2(g[i], c));
         };
         if (plain) summarise(Plain()); else summarise(Marked());
-        const Stretch own = {make_float4(A.x, b.x, A.y, b.y)};
-        segs[parity][warp][lane] = own.v;
-        sent[parity][warp][lane] = c;
-        __syncthreads();
+        chain[parity].of(warp) = Stretch{A, b};
+        back[parity].of(kWarps - 1 - warp) = Stretch{A, c};
+        const bool marked = __syncthreads_or(starts != 0);       // a start flag in the tile
         // 2. the state that enters the segment, and c that enters it from behind
-#pragma unroll
-        for (int j = 0; j < kWarps - 1; ++j)
-            if (j < warp) h = Stretch{segs[parity][j][lane]}.of(h);
-        const auto before = [&](int j) {
-            const float4 s = segs[parity][j][lane];
-            const float2 b = sent[parity][j][lane];
-            return make_float4(s.x, b.x, s.z, b.y);
-        };
-        float2 e;
+        F2 e;
         if (ranks > 1) {
-            Stretch rear = Stretch::nothing();
-#pragma unroll
-            for (int j = kWarps - 1; j > 0; --j)
-                if (j > warp) rear.follow(before(j));
-            if (warp == 0) {
-                Stretch tile = rear;
-                tile.follow(make_float4(own.v.x, c.x, own.v.z, c.y));
-                ex.send(done, at.rank, ranks, tile, lane);
-            }
-            ex.wait(done, lost, p.status);
+            if (warp == 0) ex.send(rounds - 1 - round, at.rank, ranks, back[parity].all(), lane);
+            ex.wait(rounds - 1 - round, lost, p.status);
             for (int q = ranks - 1; q >= 0; --q) {
                 if (q == at.rank) e = carry;
-                const Stretch tile = {ex.tiles[parity][q][lane]};
-                carry = tile.of(carry);
+                carry = ex.tiles[(rounds - 1 - round) & 1][q][lane].of(carry);
             }
-            e = rear.of(e);
         } else {
             e = carried[parity][lane];
-#pragma unroll
-            for (int j = kWarps - 1; j > 0; --j)
-                if (j > warp) e = Stretch{before(j)}.of(e);
         }
+        h = chain[parity].follow(h, warp, marked);
+        e = back[parity].follow(e, kWarps - 1 - warp, marked);
         // 3. the states again, and in the place of x what df is dx times of; then back through the segment
+        const long long tile_at = (((long long)at.bi * p.T + tile) * p.C + c0) * (long long)sizeof(T);
+        char *const to_x = (char*)dx + tile_at, *const to_f = (char*)df + tile_at;
         const auto walk = [&](auto kind) {
 #pragma unroll
             for (int i = 0; i < kSeg; ++i) {
                 const bool start = !kind.value && ((starts >> i) & 1u);
-                const float2 in = start ? both(0.f) : h, u = increment(i);
+                const F2 in = start ? both(0.f) : h, u = increment(i);
                 h = start ? u : fma2(a[i], h, u);
                 if (kGate == kSigmoidGate) x[i] = mul2(fma2(x[i], both(-1.f), in), a[i]);
                 else x[i] = start ? both(0.f) : mul2(mul2(in, w[i]), both(-1.f));
             }
-            const size_t last = base + (size_t)(t0 + kSeg - 1) * p.C;
-            T *to_x = dx + last, *to_f = df + last;
+            uint32_t off = own_off;
 #pragma unroll
-            for (int i = kSeg - 1; i >= 0; --i, to_x -= p.C, to_f -= p.C) {
-                const float2 d = add2(g[i], e), o = kGate == kSigmoidGate ? mul2(d, w[i]) : d, of = mul2(o, x[i]);
+            for (int i = kSeg - 1; i >= 0; --i, off -= down) {
+                const F2 d = add2(g[i], e), o = kGate == kSigmoidGate ? mul2(d, w[i]) : d, of = mul2(o, x[i]);
                 if (kind.value || i < n) {
-                    put<T, kPiece>(to_x, o.x, o.y, at.channels);
-                    put<T, kPiece>(to_f, of.x, of.y, at.channels);
+                    put<T, kPiece>((T*)(to_x + off), o, at.channels);
+                    put<T, kPiece>((T*)(to_f + off), of, at.channels);
                 }
                 e = !kind.value && ((starts >> i) & 1u) ? both(0.f) : mul2(a[i], d);
             }
         };
         if (plain) walk(Plain()); else walk(Marked());
-        if (t0 == 0) put_state(ds0 + at.state, at.L == 0 ? make_float2(e.x + gstate.x, e.y + gstate.y) : e, at.channels);
+        if (t0 == 0) put_state(ds0 + state, at.L == 0 ? add2(e, gstate) : e, at.channels);
         if (ranks == 1 && warp == 0) carried[parity ^ 1][lane] = e;
     }
     ex.close(ranks);
@@ -468,14 +493,15 @@ gated_step_kernel(int B, int C, const T* x, long long x_stride, const T* f, long
 #pragma unroll
     for (int v = 0; v < V; v += 2) {
         const int v1 = v + (V > 1);        // (one channel: twice the same)
-        const float2 x2 = make_float2(to_f32(rx.q[v]), to_f32(rx.q[v1])), s2 = make_float2(rs.q[v], rs.q[v1]);
-        float2 a, w;
-        gate_of<T, kGate>(make_float2(to_f32(rf.q[v]), to_f32(rf.q[v1])), a, w);
-        const float2 u = kGate == kSigmoidGate ? mul2(w, x2) : x2, out = start ? u : fma2(a, s2, u);
+        const F2 x2 = make_f2(to_f32(rx.q[v]), to_f32(rx.q[v1])), s2 = make_f2(rs.q[v], rs.q[v1]);
+        F2 a, w;
+        gate_of<T, kGate>(make_f2(to_f32(rf.q[v]), to_f32(rf.q[v1])), a, w);
+        const F2 u = kGate == kSigmoidGate ? mul2(w, x2) : x2;
+        const float2 out = parts(start ? u : fma2(a, s2, u));
         ry.q[v] = from_f32<T>(out.x);
         ry.q[v1] = from_f32<T>(out.y);
-        rh.q[v] = keep ? s2.x : out.x;
-        rh.q[v1] = keep ? s2.y : out.y;
+        rh.q[v] = keep ? rs.q[v] : out.x;
+        rh.q[v1] = keep ? rs.q[v1] : out.y;
     }
     *(Few<T, V>*)(y + (size_t)bi * C + c) = ry;
     *(Few<float, V>*)(s_out + bi * s_out_stride + c) = rh;
@@ -492,7 +518,7 @@ struct Residency {
             const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             for (int n = 1; n <= kMaxCluster; ++n) {
                 cudaLaunchAttribute attr[1];
-                cudaLaunchConfig_t cfg = config(attr, n, n, smem, nullptr);
+                cudaLaunchConfig_t cfg = config(attr, n, dim3(n), smem, nullptr);
                 int fit = 0;
                 if (cudaOccupancyMaxActiveClusters(&fit, kern, &cfg) != cudaSuccess) {
                     (void)cudaGetLastError();
@@ -504,11 +530,11 @@ struct Residency {
         });
         return ok ? clusters[dev] : nullptr;
     }
-    static cudaLaunchConfig_t config(cudaLaunchAttribute* attr, int ranks, unsigned grid, size_t smem, cudaStream_t st) {
+    static cudaLaunchConfig_t config(cudaLaunchAttribute* attr, int ranks, dim3 grid, size_t smem, cudaStream_t st) {
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(grid);
+        cfg.gridDim = grid;
         cfg.blockDim = dim3(kWarps * 32);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = st;
@@ -530,12 +556,13 @@ int ranks_of(const int* resident, long long units, int tiles) {
     return best;
 }
 template <typename Kernel, typename... Args>
-int launch(Residency& residency, Kernel kern, cudaStream_t st, int B, const Problem& p, int tile, size_t smem, Args... args) {
+int launch(Residency& residency, Kernel kern, cudaStream_t st, const Problem& p, int tile, size_t smem, Args... args) {
     const int* const resident = residency.of(kern, smem);
     if (resident == nullptr) return B200WKV_ELAUNCH;
-    const int units = B * p.slabs, ranks = ranks_of(resident, units, (p.T + tile - 1) / tile);
+    const int slabs = (p.C + kWide - 1) / kWide, ranks = ranks_of(resident, (long long)p.B * slabs, (p.T + tile - 1) / tile);
+    const unsigned y = p.B < 65535 ? p.B : 65535;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = Residency::config(attr, ranks, (unsigned)units * ranks, smem, st);
+    const cudaLaunchConfig_t cfg = Residency::config(attr, ranks, dim3((unsigned)slabs * ranks, y, (p.B + y - 1) / y), smem, st);
     return cudaLaunchKernelEx(&cfg, kern, p, args...) == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
 }
 // The widest pieces that every row of these begins on.
@@ -546,15 +573,15 @@ int piece_of(int C, int element, std::initializer_list<const void*> streams, std
     return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
 }
 
-template <typename T, int kGate, int kPiece> int fwd(cudaStream_t st, int B, const Problem& p, void* y, float* s_out, float* kept) {
+template <typename T, int kGate, int kPiece> int fwd(cudaStream_t st, const Problem& p, void* y, float* s_out, float* kept) {
     static Residency once;
     constexpr int kTile = kFwdSeg<T> * kWarps;
-    return launch(once, gated_fwd_kernel<T, kGate, kPiece>, st, B, p, kTile, (size_t)kStages * 2 * kTile * kWide * sizeof(T), (T*)y, s_out, kept);
+    return launch(once, gated_fwd_kernel<T, kGate, kPiece>, st, p, kTile, (size_t)kStages * 2 * kTile * kWide * sizeof(T), (T*)y, s_out, kept);
 }
 template <typename T, int kGate, int kPiece>
-int bwd(cudaStream_t st, int B, const Problem& p, const void* gy, const float* gs, const float* kept, void* dx, void* df, float* ds0) {
+int bwd(cudaStream_t st, const Problem& p, const void* gy, const float* gs, const float* kept, void* dx, void* df, float* ds0) {
     static Residency once;
-    return launch(once, gated_bwd_kernel<T, kGate, kPiece>, st, B, p, kKept, (size_t)kStages * 3 * kKept * kWide * sizeof(T), (const T*)gy, gs, kept,
+    return launch(once, gated_bwd_kernel<T, kGate, kPiece>, st, p, kKept, (size_t)kStages * 3 * kKept * kWide * sizeof(T), (const T*)gy, gs, kept,
                   (T*)dx, (T*)df, ds0);
 }
 // calls `go` with the element type, the gate and the piece as template arguments
@@ -577,18 +604,18 @@ size_t gated_residual_bytes(int B, int T, int C) { return (size_t)B * ((T + kKep
 int gated_fwd(cudaStream_t st, int dtype, int gate, int B, int T, int C, const void* x, long long x_batch, long long x_token, const void* f,
               long long f_batch, long long f_token, const float* s0, const uint32_t* length, const uint8_t* ns, void* y, float* s_out,
               void* residual) {
-    const Problem p = {T, C, (C + kWide - 1) / kWide, {x, x_batch, x_token}, {f, f_batch, f_token}, s0, length, ns, wkv7_chunk_status_word()};
+    const Problem p = {B, T, C, {x, x_batch, x_token}, {f, f_batch, f_token}, s0, length, ns, wkv7_chunk_status_word()};
     const int piece = piece_of(C, dtype == B200WKV_F32 ? 4 : 2, {x, f, y}, {x_batch, x_token, f_batch, f_token});
-    return dtype == B200WKV_F32 ? B200WKV_GATED_PIECE(fwd, float, piece, st, B, p, y, s_out, (float*)residual)
-                                : B200WKV_GATED_PIECE(fwd, __nv_bfloat16, piece, st, B, p, y, s_out, (float*)residual);
+    return dtype == B200WKV_F32 ? B200WKV_GATED_PIECE(fwd, float, piece, st, p, y, s_out, (float*)residual)
+                                : B200WKV_GATED_PIECE(fwd, __nv_bfloat16, piece, st, p, y, s_out, (float*)residual);
 }
 int gated_bwd(cudaStream_t st, int dtype, int gate, int B, int T, int C, const void* x, long long x_batch, long long x_token, const void* f,
               long long f_batch, long long f_token, const uint32_t* length, const uint8_t* ns, const void* gy, const float* gs,
               const void* residual, void* dx, void* df, float* ds0) {
-    const Problem p = {T, C, (C + kWide - 1) / kWide, {x, x_batch, x_token}, {f, f_batch, f_token}, nullptr, length, ns, wkv7_chunk_status_word()};
+    const Problem p = {B, T, C, {x, x_batch, x_token}, {f, f_batch, f_token}, nullptr, length, ns, wkv7_chunk_status_word()};
     const int piece = piece_of(C, dtype == B200WKV_F32 ? 4 : 2, {x, f, gy, dx, df}, {x_batch, x_token, f_batch, f_token});
-    return dtype == B200WKV_F32 ? B200WKV_GATED_PIECE(bwd, float, piece, st, B, p, gy, gs, (const float*)residual, dx, df, ds0)
-                                : B200WKV_GATED_PIECE(bwd, __nv_bfloat16, piece, st, B, p, gy, gs, (const float*)residual, dx, df, ds0);
+    return dtype == B200WKV_F32 ? B200WKV_GATED_PIECE(bwd, float, piece, st, p, gy, gs, (const float*)residual, dx, df, ds0)
+                                : B200WKV_GATED_PIECE(bwd, __nv_bfloat16, piece, st, p, gy, gs, (const float*)residual, dx, df, ds0);
 }
 int gated_step(cudaStream_t st, int dtype, int gate, int B, int C, const void* x, long long x_stride, const void* f, long long f_stride,
                const float* s, long long s_stride, const uint32_t* length, const uint8_t* ns, void* y, float* s_out, long long s_out_stride) {

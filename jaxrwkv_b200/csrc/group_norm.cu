@@ -28,7 +28,7 @@ struct Params {                            // weight or bias; p NULL: ones or ze
     const void* p;
     int f32;
     // N from the c-th on, as pairs (N == 1: the same in both places); 16-byte loads where `vectors`
-    template <int N> __device__ __forceinline__ void load(int c, bool vectors, float otherwise, float2* to) const {
+    template <int N> __device__ __forceinline__ void load(int c, bool vectors, float otherwise, F2* to) const {
         if (p == nullptr) {
 #pragma unroll
             for (int i = 0; i < (N + 1) / 2; ++i) to[i] = both(otherwise);
@@ -38,8 +38,8 @@ struct Params {                            // weight or bias; p NULL: ones or ze
 #pragma unroll
             for (int i = 0; i < N / 4; ++i) {
                 const float4 q = ((const float4*)((const float*)p + c))[i];
-                to[2 * i] = make_float2(q.x, q.y);
-                to[2 * i + 1] = make_float2(q.z, q.w);
+                to[2 * i] = make_f2(q.x, q.y);
+                to[2 * i + 1] = make_f2(q.z, q.w);
             }
         } else if (vectors) {
 #pragma unroll
@@ -51,8 +51,8 @@ struct Params {                            // weight or bias; p NULL: ones or ze
         } else {
 #pragma unroll
             for (int i = 0; i < N / 2; ++i)
-                to[i] = f32 ? make_float2(((const float*)p)[c + 2 * i], ((const float*)p)[c + 2 * i + 1])
-                            : make_float2(__bfloat162float(((const __nv_bfloat16*)p)[c + 2 * i]), __bfloat162float(((const __nv_bfloat16*)p)[c + 2 * i + 1]));
+                to[i] = f32 ? make_f2(((const float*)p)[c + 2 * i], ((const float*)p)[c + 2 * i + 1])
+                            : make_f2(__bfloat162float(((const __nv_bfloat16*)p)[c + 2 * i]), __bfloat162float(((const __nv_bfloat16*)p)[c + 2 * i + 1]));
         }
     }
 };
@@ -73,34 +73,40 @@ struct Problem {
 // A piece of a row as it lies in memory: VEC elements, 16 bytes, or one.  As pairs of floats a single element stands in both places.
 template <typename T, int VEC> struct Piece { uint4 q; };
 template <typename T> struct Piece<T, 1> { T q; };
-template <typename T, int VEC> __device__ __forceinline__ void unpack(const Piece<T, VEC>& r, float2* v) {
+template <typename T, int VEC> __device__ __forceinline__ void unpack(const Piece<T, VEC>& r, F2* v) {
     if constexpr (VEC == 1) v[0] = both(to_f32(r.q));
     else if constexpr (sizeof(T) == 4) {
-        v[0] = make_float2(__uint_as_float(r.q.x), __uint_as_float(r.q.y));
-        v[1] = make_float2(__uint_as_float(r.q.z), __uint_as_float(r.q.w));
+        v[0] = make_f2(__uint_as_float(r.q.x), __uint_as_float(r.q.y));
+        v[1] = make_f2(__uint_as_float(r.q.z), __uint_as_float(r.q.w));
     } else {
         v[0] = unpack_pair(r.q.x); v[1] = unpack_pair(r.q.y); v[2] = unpack_pair(r.q.z); v[3] = unpack_pair(r.q.w);
     }
 }
-template <typename T, int VEC> __device__ __forceinline__ void store_piece(T* p, const float2* v) {
+template <typename T, int VEC> __device__ __forceinline__ void store_piece(T* p, const F2* v) {
     if constexpr (VEC == 1) {
-        *p = from_f32<T>(v[0].x);
+        *p = from_f32<T>(parts(v[0]).x);
     } else if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(v[0].v, v[1].v);
     } else {
         uint4 q;
         __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[i].x, v[i].y);
+        for (int i = 0; i < 4; ++i) {
+            const float2 t = parts(v[i]);
+            h[i] = __floats2bfloat162_rn(t.x, t.y);
+        }
         *reinterpret_cast<uint4*>(p) = q;
     }
 }
-template <int VEC> __device__ __forceinline__ float sum_of(float2 v) { return VEC == 1 ? v.x : v.x + v.y; }
+template <int VEC> __device__ __forceinline__ float sum_of(F2 v) {
+    const float2 t = parts(v);
+    return VEC == 1 ? t.x : t.x + t.y;
+}
 
 // act(z), and its derivative where it is asked for
-template <typename T, int kAct> __device__ __forceinline__ void activate(float2 z, float2& p, float2& dp) {
+template <typename T, int kAct> __device__ __forceinline__ void activate(F2 z, F2& p, F2& dp) {
     if (kAct == B200WKV_ACT_NONE) { p = z; dp = both(1.f); return; }
-    float2 s, r;
+    F2 s, r;
     sigmoid_pair<T>(z, s, r);
     p = kAct == B200WKV_ACT_SIGMOID ? s : mul2(z, s);
     dp = kAct == B200WKV_ACT_SIGMOID ? mul2(s, r) : mul2(s, fma2(z, r, both(1.f)));
@@ -145,7 +151,7 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
     const Place at(p);
     const int pieces = p.D / VEC, c = at.g * p.D + at.lane * VEC, step = p.team * VEC;      // channels from piece to piece
     const float inv_d = 1.f / (float)p.D;
-    float2 w[K][kPairs], b[K][kPairs];
+    F2 w[K][kPairs], b[K][kPairs];
     Piece<T, VEC> rx[K] = {}, rg[K] = {};
     bool there[K];
 #pragma unroll
@@ -177,7 +183,7 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
     const long long steps = (p.rows + p.parallel - 1) / p.parallel;
     long long row = at.first;
     for (long long i = 0; i < steps; ++i, row += p.parallel, py += (long long)p.parallel * p.C) {
-        float2 x[K][kPairs], g[K][kPairs], sums = both(0.f);
+        F2 x[K][kPairs], g[K][kPairs], sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             unpack<T, VEC>(rx[k], x[k]);
@@ -190,7 +196,7 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
         sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            float2 squares = both(0.f);
+            F2 squares = both(0.f);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) {
                 x[k][j] = add2(x[k][j], both(-mean));
@@ -203,11 +209,11 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (!there[k] || row >= p.rows) continue;
-                float2 out[kPairs];
+                F2 out[kPairs];
 #pragma unroll
                 for (int j = 0; j < kPairs; ++j) {
-                    const float2 n = fma2(mul2(x[k][j], both(rstd)), w[k][j], b[k][j]);
-                    float2 a, da;
+                    const F2 n = fma2(mul2(x[k][j], both(rstd)), w[k][j], b[k][j]);
+                    F2 a, da;
                     activate<T, act.value>(kGate ? g[k][j] : n, a, da);
                     out[j] = kGate ? mul2(n, a) : a;
                 }
@@ -229,7 +235,7 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     const Place at(p);
     const int pieces = p.D / VEC, c = at.g * p.D + at.lane * VEC, step = p.team * VEC;
     const float inv_d = 1.f / (float)p.D;
-    float2 w[K][kPairs], b[K][kPairs], dw[K][kPairs], db[K][kPairs];
+    F2 w[K][kPairs], b[K][kPairs], dw[K][kPairs], db[K][kPairs];
     Piece<T, VEC> rx[K] = {}, rg[K] = {}, rd[K] = {};
     bool there[K];
 #pragma unroll
@@ -263,7 +269,7 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     long long row = at.first;
     for (long long i = 0; i < steps; ++i, row += p.parallel, dense += (long long)p.parallel * p.C) {
         const bool on = row < p.rows;
-        float2 x[K][kPairs], g[K][kPairs], d[K][kPairs], sums = both(0.f);
+        F2 x[K][kPairs], g[K][kPairs], d[K][kPairs], sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             unpack<T, VEC>(rx[k], x[k]);
@@ -277,7 +283,7 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
         sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            float2 squares = both(0.f);
+            F2 squares = both(0.f);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) {
                 x[k][j] = add2(x[k][j], both(-mean));
@@ -286,21 +292,21 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
             if (there[k]) sums = add2(sums, squares);
         }
         const float rstd = rsqrtf(team_sum<kBlock>(sum_of<VEC>(sums), p.team, room) * inv_d + p.eps);
-        float2 s1 = both(0.f), s2 = both(0.f);          // of dxh and dxh xh
+        F2 s1 = both(0.f), s2 = both(0.f);          // of dxh and dxh xh
         const auto gradients = [&](auto act) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (!there[k] || !on) continue;
 #pragma unroll
                 for (int j = 0; j < kPairs; ++j) {
-                    const float2 xh = mul2(x[k][j], both(rstd)), n = fma2(xh, w[k][j], b[k][j]);
-                    float2 a, da;
+                    const F2 xh = mul2(x[k][j], both(rstd)), n = fma2(xh, w[k][j], b[k][j]);
+                    F2 a, da;
                     activate<T, act.value>(kGate ? g[k][j] : n, a, da);
-                    const float2 dn = mul2(d[k][j], kGate ? a : da);
+                    const F2 dn = mul2(d[k][j], kGate ? a : da);
                     if (kGate) g[k][j] = mul2(mul2(d[k][j], n), da);
                     dw[k][j] = fma2(dn, xh, dw[k][j]);
                     db[k][j] = add2(db[k][j], dn);
-                    const float2 dxh = mul2(dn, w[k][j]);
+                    const F2 dxh = mul2(dn, w[k][j]);
                     s1 = add2(s1, dxh);
                     s2 = fma2(dxh, xh, s2);
                     x[k][j] = xh;
@@ -323,7 +329,7 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     }
     if (partial == nullptr) return;
     // partial rows (parallel or one per CTA, 2, C): weight, bias
-    const auto of = [](const float2* v, int i) { return i % 2 == 0 ? v[i / 2].x : v[i / 2].y; };
+    const auto of = [](const F2* v, int i) { return i % 2 == 0 ? parts(v[i / 2]).x : parts(v[i / 2]).y; };
     if (!kBlock && p.reduce) {
         const int in_cta = threadIdx.x / p.team;
 #pragma unroll

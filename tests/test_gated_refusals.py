@@ -26,7 +26,7 @@ def fwd(lib, dtype=1, gate=0, B=1, T=4, C=8, x=A, f=A, s0=A, length=None, ns=Non
 def test_recurrence_forward(lib):
     assert fwd(lib, dtype=2) == -1
     assert fwd(lib, gate=2) == -6
-    for bad in (dict(B=0), dict(T=0), dict(C=0), dict(B=1 << 20, T=1 << 20), dict(B=1 << 16, C=1 << 16), dict(T=(1 << 30) + 1)):
+    for bad in (dict(B=0), dict(T=0), dict(C=0), dict(B=1 << 20, T=1 << 20), dict(B=1 << 16, C=1 << 16), dict(C=(1 << 22) + 1), dict(T=(1 << 30) + 1)):
         assert fwd(lib, **bad) == -2, bad
     for name in ("x", "f", "y", "s_out"):
         assert fwd(lib, **{name: None}) == -3, name

@@ -126,15 +126,32 @@ def test_a_start_flag_drops_what_is_no_number(at, dtype, gate):
     ns[:, at] = True
     clean = train(x, f, s, length, ns, gate, gs, gy)
     for value in (float("nan"), float("inf")):
-        x2, s2, gy2 = x.clone(), s.clone(), gy.clone()
-        x2[:, :at], s2[:] = value, value
+        x2, f2, s2, gy2 = x.clone(), f.clone(), s.clone(), gy.clone()
+        x2[:, :at], s2[:], f2[:, :at, ::2] = value, value, float("nan")
+        got = train(x2, f2, s2, length, ns, gate, gs, gy)
         for i in (1, 2, 3):                       # behind the flag: outputs and gradients as if nothing had been there
-            assert torch.equal(train(x2, f, s2, length, ns, gate, gs, gy)[i][:, at:], clean[i][:, at:])
+            assert torch.equal(got[i][:, at:], clean[i][:, at:])
         gy2[:, at:] = value
         got = train(x, f, s, length, ns, gate, gs * torch.tensor([[value], [1.0]], device="cuda"), gy2)
         for i in (2, 3):                          # in front of it: gradients likewise (the second's state ends at the flag)
             assert torch.equal(got[i][:, :at], clean[i][:, :at])
         assert torch.equal(got[4], clean[4])
+
+
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("at", [3, 66, 130])
+def test_a_gate_that_is_no_number_stays_in_its_channel(at, gate):
+    """Behind a flag of its own segment, in every second channel."""
+    x, f, s, length, ns, gy, gs = cuda(*inputs(2, 200, 40, gate, torch.bfloat16, seed=20, lengths=[200, 150]))
+    s[:] = float("inf")
+    ns[:, at - 1] = True
+    clean = train(x, f, s, length, ns, gate, gs, gy)
+    f2 = f.clone()
+    f2[:, at, ::2] = float("nan")
+    got = train(x, f2, s, length, ns, gate, gs, gy)
+    for i in range(5):
+        assert torch.equal(got[i][..., 1::2].nan_to_num(7.0), clean[i][..., 1::2].nan_to_num(7.0))
+    assert got[1][:, at:, ::2].isnan().all() and torch.equal(got[1][:, at - 1, ::2], clean[1][:, at - 1, ::2])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

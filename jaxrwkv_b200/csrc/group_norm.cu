@@ -22,37 +22,36 @@ namespace b200wkv {
 namespace {
 
 constexpr int kMaxPartials = 1024;         // partial rows of the parameters' gradients
-constexpr int kMaxThreads = 1024;
+constexpr int kMaxThreads = 512;
 
 struct Params {                            // weight or bias; p NULL: ones or zeros
     const void* p;
     int f32;
-    // N from the c-th on, as pairs (N == 1: the same in both places); 16-byte loads where `vectors`
-    template <int N> __device__ __forceinline__ void load(int c, bool vectors, float otherwise, F2* to) const {
+    __device__ __forceinline__ float at(int c) const { return f32 ? ((const float*)p)[c] : __bfloat162float(((const __nv_bfloat16*)p)[c]); }
+    // N from the c-th on as pairs, of which the first `valid` are there; 16-byte loads where `vectors`
+    template <int N> __device__ __forceinline__ void load(int c, int valid, bool vectors, float otherwise, F2* to) const {
         if (p == nullptr) {
 #pragma unroll
-            for (int i = 0; i < (N + 1) / 2; ++i) to[i] = both(otherwise);
-        } else if constexpr (N == 1) {
-            to[0] = both(f32 ? ((const float*)p)[c] : __bfloat162float(((const __nv_bfloat16*)p)[c]));
-        } else if (f32 && vectors) {
+            for (int i = 0; i < N / 2; ++i) to[i] = both(otherwise);
+        } else if (N % 4 == 0 && vectors) {
+            if (f32) {
 #pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const float4 q = ((const float4*)((const float*)p + c))[i];
-                to[2 * i] = make_f2(q.x, q.y);
-                to[2 * i + 1] = make_f2(q.z, q.w);
-            }
-        } else if (vectors) {
+                for (int i = 0; i < N / 4; ++i) {
+                    const ulonglong2 q = ((const ulonglong2*)((const float*)p + c))[i];
+                    to[2 * i].v = q.x;
+                    to[2 * i + 1].v = q.y;
+                }
+            } else {
 #pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const uint2 q = ((const uint2*)((const __nv_bfloat16*)p + c))[i];
-                to[2 * i] = unpack_pair(q.x);
-                to[2 * i + 1] = unpack_pair(q.y);
+                for (int i = 0; i < N / 4; ++i) {
+                    const uint2 q = ((const uint2*)((const __nv_bfloat16*)p + c))[i];
+                    to[2 * i] = unpack_pair(q.x);
+                    to[2 * i + 1] = unpack_pair(q.y);
+                }
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i)
-                to[i] = f32 ? make_f2(((const float*)p)[c + 2 * i], ((const float*)p)[c + 2 * i + 1])
-                            : make_f2(__bfloat162float(((const __nv_bfloat16*)p)[c + 2 * i]), __bfloat162float(((const __nv_bfloat16*)p)[c + 2 * i + 1]));
+            for (int i = 0; i < N / 2; ++i) to[i] = make_f2(at(c + 2 * i), 2 * i + 1 < valid ? at(c + 2 * i + 1) : 0.f);
         }
     }
 };
@@ -70,38 +69,62 @@ struct Problem {
     int reduce;                            // teams of one group within a CTA are added up (per_cta is a multiple of G)
 };
 
-// A piece of a row as it lies in memory: VEC elements, 16 bytes, or one.  As pairs of floats a single element stands in both places.
-template <typename T, int VEC> struct Piece { uint4 q; };
-template <typename T> struct Piece<T, 1> { T q; };
-template <typename T, int VEC> __device__ __forceinline__ void unpack(const Piece<T, VEC>& r, F2* v) {
-    if constexpr (VEC == 1) v[0] = both(to_f32(r.q));
-    else if constexpr (sizeof(T) == 4) {
-        v[0] = make_f2(__uint_as_float(r.q.x), __uint_as_float(r.q.y));
-        v[1] = make_f2(__uint_as_float(r.q.z), __uint_as_float(r.q.w));
-    } else {
-        v[0] = unpack_pair(r.q.x); v[1] = unpack_pair(r.q.y); v[2] = unpack_pair(r.q.z); v[3] = unpack_pair(r.q.w);
+// A piece of a row as it lies in memory: VEC adjacent elements of one load, or (kWhole false) two of one load each, of which the second may
+// lie behind the group's end and is 0 then.
+template <typename T, int VEC, bool kWhole> struct Piece {
+    static constexpr int kWords = VEC * (int)sizeof(T) / 4;
+    uint32_t q[kWords];
+    __device__ __forceinline__ void load(const T* p, bool) {
+        if constexpr (kWords == 4) {
+            const uint4 v = *(const uint4*)p;
+            q[0] = v.x; q[1] = v.y; q[2] = v.z; q[3] = v.w;
+        } else if constexpr (kWords == 2) {
+            const uint2 v = *(const uint2*)p;
+            q[0] = v.x; q[1] = v.y;
+        } else q[0] = *(const uint32_t*)p;
     }
-}
-template <typename T, int VEC> __device__ __forceinline__ void store_piece(T* p, const F2* v) {
-    if constexpr (VEC == 1) {
-        *p = from_f32<T>(parts(v[0]).x);
-    } else if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(v[0].v, v[1].v);
-    } else {
-        uint4 q;
-        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
+    __device__ __forceinline__ void unpack(F2* v) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 t = parts(v[i]);
-            h[i] = __floats2bfloat162_rn(t.x, t.y);
-        }
-        *reinterpret_cast<uint4*>(p) = q;
+        for (int i = 0; i < VEC / 2; ++i)
+            v[i] = sizeof(T) == 4 ? make_f2(__uint_as_float(q[2 * i % kWords]), __uint_as_float(q[(2 * i + 1) % kWords])) : unpack_pair(q[i % kWords]);
     }
-}
-template <int VEC> __device__ __forceinline__ float sum_of(F2 v) {
+    __device__ __forceinline__ static void store(T* p, const F2* v, bool) {
+        uint32_t w[kWords];
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            const float2 t = parts(v[i]);
+            if constexpr (sizeof(T) == 4) {
+                w[2 * i] = __float_as_uint(t.x);
+                w[2 * i + 1] = __float_as_uint(t.y);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(t.x, t.y);
+                w[i] = *(const uint32_t*)&h;
+            }
+        }
+        if constexpr (kWords == 4) *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (kWords == 2) *(uint2*)p = make_uint2(w[0], w[1]);
+        else *(uint32_t*)p = w[0];
+    }
+};
+template <typename T, int VEC> struct Piece<T, VEC, false> {
+    static_assert(VEC == 2, "two elements");
+    T q[2];
+    __device__ __forceinline__ void load(const T* p, bool second) {
+        q[0] = p[0];
+        if (second) q[1] = p[1];
+    }
+    __device__ __forceinline__ void unpack(F2* v) const { v[0] = make_f2(to_f32(q[0]), to_f32(q[1])); }
+    __device__ __forceinline__ static void store(T* p, const F2* v, bool second) {
+        const float2 t = parts(v[0]);
+        p[0] = from_f32<T>(t.x);
+        if (second) p[1] = from_f32<T>(t.y);
+    }
+};
+__device__ __forceinline__ float sum_of(F2 v) {
     const float2 t = parts(v);
-    return VEC == 1 ? t.x : t.x + t.y;
+    return t.x + t.y;
 }
+__device__ __forceinline__ F2 first_alone(F2 v) { return make_f2(parts(v).x, 0.f); }
 
 // act(z), and its derivative where it is asked for
 template <typename T, int kAct> __device__ __forceinline__ void activate(F2 z, F2& p, F2& dp) {
@@ -142,39 +165,83 @@ struct Place {
     }
 };
 
-// Registers: weight, bias and a row's values; 4 CTAs an SM where the team is a part of a warp
-template <typename T, int VEC, int K, bool kBlock, bool kGate>
-__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : VEC * K > 8 || VEC == 1 && K == 8 ? 2 : 4)
-group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
-    constexpr int kPairs = (VEC + 1) / 2;
-    __shared__ float room[kBlock ? 32 : 1];
-    const Place at(p);
-    const int pieces = p.D / VEC, c = at.g * p.D + at.lane * VEC, step = p.team * VEC;      // channels from piece to piece
-    const float inv_d = 1.f / (float)p.D;
+// The pieces of one thread: K, `step` channels apart.  kWhole false: the group's last element may be the first of a pair (`odd`).
+template <typename T, int VEC, int K, bool kWhole> struct Lane {
+    static constexpr int kPairs = VEC / 2;
+    typedef Piece<T, VEC, kWhole> P;
+    int c, step;                           // the first piece's channel in the row
+    bool there[K], second[K];              // the piece; its second element (kWhole false)
     F2 w[K][kPairs], b[K][kPairs];
-    Piece<T, VEC> rx[K] = {}, rg[K] = {};
-    bool there[K];
+    __device__ __forceinline__ Lane(const Problem& p, const Place& at) : c(at.g * p.D + at.lane * VEC), step(p.team * VEC) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        there[k] = at.at_work && at.lane + k * p.team < pieces;
-        if (there[k]) {
-            p.weight.load<VEC>(c + k * step, p.param_vectors, 1.f, w[k]);
-            p.bias.load<VEC>(c + k * step, p.param_vectors, 0.f, b[k]);
-        } else {
+        for (int k = 0; k < K; ++k) {
+            const int d = (at.lane + k * p.team) * VEC;
+            there[k] = at.at_work && d < p.D;
+            second[k] = kWhole || d + 1 < p.D;
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) w[k][i] = b[k][i] = both(0.f);
+            if (there[k]) {
+                p.weight.load<VEC>(c + k * step, p.D - d, p.param_vectors, 1.f, w[k]);
+                p.bias.load<VEC>(c + k * step, p.D - d, p.param_vectors, 0.f, b[k]);
+            }
         }
     }
-    const T* px = (const T*)p.x + at.first * p.x_stride + c;
-    const T* pg = kGate ? (const T*)p.gate + at.first * p.gate_stride + c : nullptr;
-    T* py = y + at.first * p.C + c;
-    const auto read = [&](long long row) {
+    __device__ __forceinline__ void load(P* to, const T* row) const {
 #pragma unroll
         for (int k = 0; k < K; ++k)
-            if (there[k] && row < p.rows) {
-                rx[k] = *(const Piece<T, VEC>*)(px + k * step);
-                if (kGate) rg[k] = *(const Piece<T, VEC>*)(pg + k * step);
+            if (there[k]) to[k].load(row + k * step, second[k]);
+    }
+    __device__ __forceinline__ void store(T* row, int k, const F2* v) const { P::store(row + k * step, v, second[k]); }
+    // x less its mean over the team (0 where there is nothing), and 1 / sqrt(var + eps)
+    template <bool kBlock> __device__ __forceinline__ float centre(F2 (&x)[K][kPairs], const Problem& p, float inv_d, float* room) const {
+        F2 sums = both(0.f);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) sums = add2(sums, x[k][j]);
+        const F2 less = both(-team_sum<kBlock>(sum_of(sums), p.team, room) * inv_d);
+        sums = both(0.f);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            F2 squares = both(0.f);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+                x[k][j] = add2(x[k][j], less);
+                if (!kWhole && !second[k]) x[k][j] = first_alone(x[k][j]);
+                squares = fma2(x[k][j], x[k][j], squares);
             }
+            if (there[k]) sums = add2(sums, squares);
+        }
+        return rsqrtf(team_sum<kBlock>(sum_of(sums), p.team, room) * inv_d + p.eps);
+    }
+};
+template <typename Go> __device__ __forceinline__ void by_activation(int act, Go go) {
+    if (act == B200WKV_ACT_SILU) go(std::integral_constant<int, B200WKV_ACT_SILU>());
+    else if (act == B200WKV_ACT_SIGMOID) go(std::integral_constant<int, B200WKV_ACT_SIGMOID>());
+    else go(std::integral_constant<int, B200WKV_ACT_NONE>());
+}
+
+// CTAs of 256 threads an SM for the registers of a kernel: weight, bias, a row's values and the next row's as they lie in memory
+constexpr int fwd_ctas(int elements, int bytes, bool gate) { return elements <= 4 || (elements <= 8 && bytes <= 16) ? 4 : elements <= 8 || !gate ? 3 : 2; }
+__host__ __device__ constexpr int bwd_ctas(int elements) { return elements <= 4 ? 3 : elements <= 8 ? 2 : 1; }
+
+template <typename T, int VEC, int K, bool kWhole, bool kBlock, bool kGate>
+__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : fwd_ctas(VEC * K, kWhole ? VEC * K * (int)sizeof(T) : 32, kGate))
+group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
+    typedef Lane<T, VEC, K, kWhole> L;
+    __shared__ float room[kBlock ? 32 : 1];
+    const Place at(p);
+    const L my(p, at);
+    const float inv_d = 1.f / (float)p.D;
+    typename L::P rx[K] = {}, rg[K] = {};
+    const T* px = (const T*)p.x + at.first * p.x_stride + my.c;
+    const T* pg = kGate ? (const T*)p.gate + at.first * p.gate_stride + my.c : nullptr;
+    T* py = y + at.first * p.C + my.c;
+    const auto read = [&](long long row) {
+        if (row < p.rows) {
+            my.load(rx, px);
+            if (kGate) my.load(rg, pg);
+        }
         px += p.parallel * p.x_stride;
         if (kGate) pg += p.parallel * p.gate_stride;
     };
@@ -183,83 +250,58 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
     const long long steps = (p.rows + p.parallel - 1) / p.parallel;
     long long row = at.first;
     for (long long i = 0; i < steps; ++i, row += p.parallel, py += (long long)p.parallel * p.C) {
-        F2 x[K][kPairs], g[K][kPairs], sums = both(0.f);
+        F2 x[K][L::kPairs], g[K][L::kPairs];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            unpack<T, VEC>(rx[k], x[k]);
-            if (kGate) unpack<T, VEC>(rg[k], g[k]);
-#pragma unroll
-            for (int j = 0; j < kPairs; ++j) sums = add2(sums, x[k][j]);
+            rx[k].unpack(x[k]);
+            if (kGate) rg[k].unpack(g[k]);
         }
         read(row + p.parallel);
-        const float mean = team_sum<kBlock>(sum_of<VEC>(sums), p.team, room) * inv_d;
-        sums = both(0.f);
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            F2 squares = both(0.f);
-#pragma unroll
-            for (int j = 0; j < kPairs; ++j) {
-                x[k][j] = add2(x[k][j], both(-mean));
-                squares = fma2(x[k][j], x[k][j], squares);
-            }
-            if (there[k]) sums = add2(sums, squares);
-        }
-        const float rstd = rsqrtf(team_sum<kBlock>(sum_of<VEC>(sums), p.team, room) * inv_d + p.eps);
-        const auto finish = [&](auto act) {
+        const F2 rstd = both(my.template centre<kBlock>(x, p, inv_d, room));
+        by_activation(p.act, [&](auto act) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (!there[k] || row >= p.rows) continue;
-                F2 out[kPairs];
+                if (!my.there[k] || row >= p.rows) continue;
+                F2 out[L::kPairs];
 #pragma unroll
-                for (int j = 0; j < kPairs; ++j) {
-                    const F2 n = fma2(mul2(x[k][j], both(rstd)), w[k][j], b[k][j]);
+                for (int j = 0; j < L::kPairs; ++j) {
+                    const F2 n = fma2(mul2(x[k][j], rstd), my.w[k][j], my.b[k][j]);
                     F2 a, da;
                     activate<T, act.value>(kGate ? g[k][j] : n, a, da);
                     out[j] = kGate ? mul2(n, a) : a;
                 }
-                store_piece<T, VEC>(py + k * step, out);
+                my.store(py, k, out);
             }
-        };
-        if (p.act == B200WKV_ACT_SILU) finish(std::integral_constant<int, B200WKV_ACT_SILU>());
-        else if (p.act == B200WKV_ACT_SIGMOID) finish(std::integral_constant<int, B200WKV_ACT_SIGMOID>());
-        else finish(std::integral_constant<int, B200WKV_ACT_NONE>());
+        });
     }
 }
 
-template <typename T, int VEC, int K, bool kBlock, bool kGate>
-__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : VEC * K > 8 || VEC == 1 && K == 8 ? 1 : 2)
+template <typename T, int VEC, int K, bool kWhole, bool kBlock, bool kGate>
+__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : bwd_ctas(VEC * K))
 group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ partial) {
-    constexpr int kPairs = (VEC + 1) / 2;
+    typedef Lane<T, VEC, K, kWhole> L;
+    constexpr int kPairs = L::kPairs;
     __shared__ float room[kBlock ? 32 : 1];
-    __shared__ float both_sums[kBlock ? 1 : 256 * VEC];
+    __shared__ float both_sums[kBlock ? 1 : 2 * 256 * VEC];
     const Place at(p);
-    const int pieces = p.D / VEC, c = at.g * p.D + at.lane * VEC, step = p.team * VEC;
+    const L my(p, at);
     const float inv_d = 1.f / (float)p.D;
-    F2 w[K][kPairs], b[K][kPairs], dw[K][kPairs], db[K][kPairs];
-    Piece<T, VEC> rx[K] = {}, rg[K] = {}, rd[K] = {};
-    bool there[K];
+    F2 dw[K][kPairs], db[K][kPairs];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        there[k] = at.at_work && at.lane + k * p.team < pieces;
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) w[k][i] = b[k][i] = dw[k][i] = db[k][i] = both(0.f);
-        if (there[k]) {
-            p.weight.load<VEC>(c + k * step, p.param_vectors, 1.f, w[k]);
-            p.bias.load<VEC>(c + k * step, p.param_vectors, 0.f, b[k]);
-        }
-    }
-    const T* px = (const T*)p.x + at.first * p.x_stride + c;
-    const T* pg = kGate ? (const T*)p.gate + at.first * p.gate_stride + c : nullptr;
-    const T* pd = gy + at.first * p.C + c;
-    long long dense = at.first * p.C + c;
+        for (int i = 0; i < kPairs; ++i) dw[k][i] = db[k][i] = both(0.f);
+    typename L::P rx[K] = {}, rg[K] = {}, rd[K] = {};
+    const T* px = (const T*)p.x + at.first * p.x_stride + my.c;
+    const T* pg = kGate ? (const T*)p.gate + at.first * p.gate_stride + my.c : nullptr;
+    const T* pd = gy + at.first * p.C + my.c;
+    long long dense = at.first * p.C + my.c;
     const auto read = [&](long long row) {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (there[k] && row < p.rows) {
-                rx[k] = *(const Piece<T, VEC>*)(px + k * step);
-                rd[k] = *(const Piece<T, VEC>*)(pd + k * step);
-                if (kGate) rg[k] = *(const Piece<T, VEC>*)(pg + k * step);
-            }
+        if (row < p.rows) {
+            my.load(rx, px);
+            my.load(rd, pd);
+            if (kGate) my.load(rg, pg);
+        }
         px += p.parallel * p.x_stride;
         pd += (long long)p.parallel * p.C;
         if (kGate) pg += p.parallel * p.gate_stride;
@@ -269,93 +311,80 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     long long row = at.first;
     for (long long i = 0; i < steps; ++i, row += p.parallel, dense += (long long)p.parallel * p.C) {
         const bool on = row < p.rows;
-        F2 x[K][kPairs], g[K][kPairs], d[K][kPairs], sums = both(0.f);
+        F2 x[K][kPairs], g[K][kPairs], d[K][kPairs];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            unpack<T, VEC>(rx[k], x[k]);
-            unpack<T, VEC>(rd[k], d[k]);
-            if (kGate) unpack<T, VEC>(rg[k], g[k]);
-#pragma unroll
-            for (int j = 0; j < kPairs; ++j) sums = add2(sums, x[k][j]);
+            rx[k].unpack(x[k]);
+            rd[k].unpack(d[k]);
+            if (kGate) rg[k].unpack(g[k]);
         }
         read(row + p.parallel);
-        const float mean = team_sum<kBlock>(sum_of<VEC>(sums), p.team, room) * inv_d;
-        sums = both(0.f);
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            F2 squares = both(0.f);
-#pragma unroll
-            for (int j = 0; j < kPairs; ++j) {
-                x[k][j] = add2(x[k][j], both(-mean));
-                squares = fma2(x[k][j], x[k][j], squares);
-            }
-            if (there[k]) sums = add2(sums, squares);
-        }
-        const float rstd = rsqrtf(team_sum<kBlock>(sum_of<VEC>(sums), p.team, room) * inv_d + p.eps);
-        F2 s1 = both(0.f), s2 = both(0.f);          // of dxh and dxh xh
-        const auto gradients = [&](auto act) {
+        const F2 rstd = both(my.template centre<kBlock>(x, p, inv_d, room));
+        F2 s1 = both(0.f), s2 = both(0.f);                // of dxh and dxh xh
+        by_activation(p.act, [&](auto act) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (!there[k] || !on) continue;
+                if (!my.there[k] || !on) continue;
 #pragma unroll
                 for (int j = 0; j < kPairs; ++j) {
-                    const F2 xh = mul2(x[k][j], both(rstd)), n = fma2(xh, w[k][j], b[k][j]);
+                    const F2 xh = mul2(x[k][j], rstd), n = fma2(xh, my.w[k][j], my.b[k][j]);
                     F2 a, da;
                     activate<T, act.value>(kGate ? g[k][j] : n, a, da);
-                    const F2 dn = mul2(d[k][j], kGate ? a : da);
+                    F2 dn = mul2(d[k][j], kGate ? a : da);
                     if (kGate) g[k][j] = mul2(mul2(d[k][j], n), da);
+                    if (!kWhole && !my.second[k]) dn = first_alone(dn);
                     dw[k][j] = fma2(dn, xh, dw[k][j]);
                     db[k][j] = add2(db[k][j], dn);
-                    const F2 dxh = mul2(dn, w[k][j]);
+                    const F2 dxh = mul2(dn, my.w[k][j]);
                     s1 = add2(s1, dxh);
                     s2 = fma2(dxh, xh, s2);
                     x[k][j] = xh;
                     d[k][j] = dxh;
                 }
             }
-        };
-        if (p.act == B200WKV_ACT_SILU) gradients(std::integral_constant<int, B200WKV_ACT_SILU>());
-        else if (p.act == B200WKV_ACT_SIGMOID) gradients(std::integral_constant<int, B200WKV_ACT_SIGMOID>());
-        else gradients(std::integral_constant<int, B200WKV_ACT_NONE>());
-        const float m1 = team_sum<kBlock>(sum_of<VEC>(s1), p.team, room) * inv_d, m2 = team_sum<kBlock>(sum_of<VEC>(s2), p.team, room) * inv_d;
+        });
+        const F2 m1 = both(-team_sum<kBlock>(sum_of(s1), p.team, room) * inv_d), m2 = both(-team_sum<kBlock>(sum_of(s2), p.team, room) * inv_d);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            if (!there[k] || !on) continue;
-            if (kGate) store_piece<T, VEC>(dgate + dense + k * step, g[k]);
+            if (!my.there[k] || !on) continue;
+            if (kGate) my.store(dgate + dense, k, g[k]);
 #pragma unroll
-            for (int j = 0; j < kPairs; ++j) d[k][j] = mul2(fma2(x[k][j], both(-m2), add2(d[k][j], both(-m1))), both(rstd));
-            store_piece<T, VEC>(dx + dense + k * step, d[k]);
+            for (int j = 0; j < kPairs; ++j) d[k][j] = mul2(fma2(x[k][j], m2, add2(d[k][j], m1)), rstd);
+            my.store(dx + dense, k, d[k]);
         }
     }
     if (partial == nullptr) return;
     // partial rows (parallel or one per CTA, 2, C): weight, bias
     const auto of = [](const F2* v, int i) { return i % 2 == 0 ? parts(v[i / 2]).x : parts(v[i / 2]).y; };
-    if (!kBlock && p.reduce) {
-        const int in_cta = threadIdx.x / p.team;
+    if (!kBlock && p.reduce) {             // teams of one group within the CTA are added first, a column a thread
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            __syncthreads();
 #pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                __syncthreads();
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) both_sums[threadIdx.x * VEC + v] = of(which == 0 ? dw[k] : db[k], v);
-                __syncthreads();
-                if (in_cta < p.G && there[k])              // the first team of its group adds the others
-                    for (int v = 0; v < VEC; ++v) {
-                        float t = 0.f;
-                        for (int j = in_cta; j < p.per_cta; j += p.G) t += both_sums[(j * p.team + at.lane) * VEC + v];
-                        partial[((size_t)blockIdx.x * 2 + which) * p.C + c + k * step + v] = t;
-                    }
+            for (int v = 0; v < VEC; ++v) {
+                both_sums[threadIdx.x * VEC + v] = of(dw[k], v);
+                both_sums[(256 + threadIdx.x) * VEC + v] = of(db[k], v);
             }
+            __syncthreads();
+            const int width = p.team * VEC, columns = 2 * p.G * width;         // of this k
+            for (int t = threadIdx.x; t < columns; t += 256) {
+                const int which = t / (p.G * width), g = t % (p.G * width) / width, d = t % width, c = d + k * width;
+                if (c >= p.D) continue;
+                float sum = 0.f;
+                for (int j = g; j < p.per_cta; j += p.G) sum += both_sums[which * 256 * VEC + j * width + d];
+                partial[((size_t)blockIdx.x * 2 + which) * p.C + g * p.D + c] = sum;
+            }
+        }
         return;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k)
-        if (there[k]) {
+        if (my.there[k]) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                partial[((size_t)at.first * 2) * p.C + c + k * step + v] = of(dw[k], v);
-                partial[((size_t)at.first * 2 + 1) * p.C + c + k * step + v] = of(db[k], v);
+                if (v == 1 && !my.second[k]) continue;
+                partial[((size_t)at.first * 2) * p.C + my.c + k * my.step + v] = of(dw[k], v);
+                partial[((size_t)at.first * 2 + 1) * p.C + my.c + k * my.step + v] = of(db[k], v);
             }
         }
 }
@@ -384,22 +413,28 @@ __global__ void __launch_bounds__(512) group_norm_sums_kernel(const float* parti
     else ((__nv_bfloat16*)to)[at] = __float2bfloat16_rn(t);
 }
 
-// How a call is cut: pieces of 16 bytes where rows and group fit them, else single elements; a team as narrow as covers the group.
+// How a call is cut.  Pieces of 16 bytes where rows and groups fit them, else pairs; a team as narrow as covers the group with K pieces a
+// thread, which keeps the shuffles few; a whole CTA where the group is wider than a warp with K.
 struct Plan {
     int vec, k, block, grid;
+    bool whole;
 };
-Plan plan_of(Problem& p, int element, bool aligned, int ctas_per_sm) {
+// `aligned`: bytes that every row and pointer begins on.
+Plan plan_of(Problem& p, int element, int aligned, bool forward) {
     Plan q;
     const int wide = 16 / element;
-    q.vec = aligned && p.D % wide == 0 && p.C % wide == 0 ? wide : 1;
-    const int pieces = p.D / q.vec, most = q.vec == 1 ? 8 : 2;
-    if (pieces <= 32 * most) {
-        q.k = pieces <= 32 ? 1 : q.vec == 1 ? (pieces <= 64 ? 2 : 8) : 2;
+    q.vec = aligned >= 16 && p.D % wide == 0 ? wide : 2;
+    q.whole = q.vec == wide || (aligned >= 2 * element && p.D % 2 == 0);
+    const int pieces = (p.D + q.vec - 1) / q.vec;
+    if (q.vec == wide) q.k = pieces <= 32 ? 1 : 2;
+    else q.k = 4;
+    if (pieces <= 32 * q.k) {
+        q.block = 256;
         p.team = 1;
         while (p.team * q.k < pieces) p.team *= 2;
-        q.block = 256;
     } else {
-        q.k = pieces <= kMaxThreads ? 1 : q.vec == 1 ? 8 : 2;
+        if (q.vec == wide) q.k = pieces <= kMaxThreads ? 1 : pieces <= 2 * kMaxThreads ? 2 : 4;
+        else q.k = pieces <= 4 * kMaxThreads ? 4 : 8;
         q.block = ((pieces + q.k - 1) / q.k + 31) / 32 * 32;
         p.team = q.block;
     }
@@ -407,10 +442,13 @@ Plan plan_of(Problem& p, int element, bool aligned, int ctas_per_sm) {
     p.reduce = p.G * 4 <= teams;
     p.per_cta = p.reduce ? teams / p.G * p.G : teams;
     const long long all = p.rows * p.G;                  // rows of groups
-    const long long most_ctas = (long long)sm_count_of_current_device() * ctas_per_sm;
+    // as many threads as the device has room for: a backward keeps its parameters' sums, so its CTAs are no more than are resident
+    const int threads = forward ? 2048 : 256 * bwd_ctas(q.vec * q.k) < 512 ? 512 : 256 * bwd_ctas(q.vec * q.k), ctas = threads > q.block ? threads / q.block : 1;
+    const long long most_ctas = (long long)sm_count_of_current_device() * (ctas < 32 ? ctas : 32);
     long long grid = (all + p.per_cta - 1) / p.per_cta;
     grid = grid < most_ctas ? grid : most_ctas;
     if (p.reduce) {
+        grid = grid < kMaxPartials ? grid : kMaxPartials;
         p.parallel = (int)(grid * (p.per_cta / p.G));
     } else {
         long long parallel = grid * p.per_cta / p.G;
@@ -422,42 +460,52 @@ Plan plan_of(Problem& p, int element, bool aligned, int ctas_per_sm) {
     q.grid = (int)grid;
     return q;
 }
-bool on_16(std::initializer_list<const void*> ps, std::initializer_list<long long> strides, int element) {
-    uintptr_t bits = 0;
+int aligned_to(std::initializer_list<const void*> ps, std::initializer_list<long long> strides, int element) {
+    uintptr_t bits = 16;
     for (const void* q : ps) bits |= reinterpret_cast<uintptr_t>(q);
     for (long long s : strides) bits |= (uintptr_t)s * element;
-    return bits % 16 == 0;
+    return (int)(bits & (0 - bits));
 }
 // `go` for the cut of a plan
 template <typename T, typename Go> int dispatch(const Plan& q, const Problem& p, Go go) {
     constexpr int kWide = 16 / sizeof(T);
+    typedef std::true_type Yes;
+    typedef std::false_type No;
+    const auto gated = [&](auto vec, auto k, auto whole, auto block) {
+        return p.gate != nullptr ? go(vec, k, whole, block, Yes()) : go(vec, k, whole, block, No());
+    };
     typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, 2> Two;
+    typedef std::integral_constant<int, 4> Four;
     typedef std::integral_constant<int, 8> Eight;
     typedef std::integral_constant<int, kWide> Wide;
-    const auto gated = [&](auto vec, auto k, auto block) {
-        return p.gate != nullptr ? go(vec, k, block, std::true_type()) : go(vec, k, block, std::false_type());
-    };
-    const auto shaped = [&](auto vec, auto k) {
-        return p.team > 32 ? gated(vec, k, std::true_type()) : gated(vec, k, std::false_type());
-    };
-    if (q.vec > 1) return q.k == 1 ? shaped(Wide(), One()) : shaped(Wide(), Two());
-    return q.k == 1 ? shaped(One(), One()) : q.k == 2 ? gated(One(), Two(), std::false_type()) : shaped(One(), Eight());
+    const bool block = p.team > 32;
+    if (q.vec == kWide) {
+        if (!block) return q.k == 1 ? gated(Wide(), One(), Yes(), No()) : gated(Wide(), Two(), Yes(), No());
+        if (q.k == 1) return gated(Wide(), One(), Yes(), Yes());
+        if constexpr (sizeof(T) == 4) {                  // (in 16 bits two pieces a thread cover the widest group)
+            if (q.k == 4) return gated(Wide(), Four(), Yes(), Yes());
+        }
+        return gated(Wide(), Two(), Yes(), Yes());
+    }
+    if (q.whole) return !block ? gated(Two(), Four(), Yes(), No()) : q.k == 4 ? gated(Two(), Four(), Yes(), Yes()) : gated(Two(), Eight(), Yes(), Yes());
+    return !block ? gated(Two(), Four(), No(), No()) : q.k == 4 ? gated(Two(), Four(), No(), Yes()) : gated(Two(), Eight(), No(), Yes());
 }
 template <typename T> int fwd(cudaStream_t st, Problem p, void* y) {
-    const Plan q = plan_of(p, sizeof(T), on_16({p.x, p.gate, y}, {p.x_stride, p.gate_stride}, sizeof(T)), 8);
-    return dispatch<T>(q, p, [&](auto vec, auto k, auto block, auto gate) {
-        group_norm_fwd_kernel<T, vec.value, k.value, block.value, gate.value><<<q.grid, q.block, 0, st>>>(p, (T*)y);
+    const Plan q = plan_of(p, sizeof(T), aligned_to({p.x, p.gate, y}, {p.x_stride, p.gate_stride, p.C}, sizeof(T)), true);
+    return dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto gate) {
+        group_norm_fwd_kernel<T, vec.value, k.value, whole.value, block.value, gate.value><<<q.grid, q.block, 0, st>>>(p, (T*)y);
         return cudaGetLastError() == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
     });
 }
 template <typename T>
 int bwd(cudaStream_t st, Problem p, const void* gy, void* dx, void* dgate, void* dweight, void* dbias, float* partial) {
-    const Plan q = plan_of(p, sizeof(T), on_16({p.x, p.gate, gy, dx, dgate}, {p.x_stride, p.gate_stride}, sizeof(T)), 2);
+    const Plan q = plan_of(p, sizeof(T), aligned_to({p.x, p.gate, gy, dx, dgate}, {p.x_stride, p.gate_stride, p.C}, sizeof(T)), false);
     const bool params = dweight != nullptr || dbias != nullptr;
     if (!params) partial = nullptr;
-    const int status = dispatch<T>(q, p, [&](auto vec, auto k, auto block, auto gate) {
-        group_norm_bwd_kernel<T, vec.value, k.value, block.value, gate.value><<<q.grid, q.block, 0, st>>>(p, (const T*)gy, (T*)dx, (T*)dgate, partial);
+    const int status = dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto gate) {
+        group_norm_bwd_kernel<T, vec.value, k.value, whole.value, block.value, gate.value>
+            <<<q.grid, q.block, 0, st>>>(p, (const T*)gy, (T*)dx, (T*)dgate, partial);
         return cudaGetLastError() == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
     });
     if (status != B200WKV_OK || !params) return status;
@@ -469,7 +517,7 @@ Problem problem(long long rows, int C, int groups, float eps, int act, const voi
                 int param_dtype, const void* gate, long long gate_stride) {
     const int f32 = param_dtype == B200WKV_F32;
     return {rows, C, groups, C / groups, act, eps, x, gate, x_stride, gate != nullptr ? gate_stride : 0, {weight, f32}, {bias, f32}, 0, 0, 0,
-            on_16({weight, bias}, {}, 4), 0};
+            aligned_to({weight, bias}, {}, 1) >= 16, 0};
 }
 }  // namespace
 

@@ -17,6 +17,7 @@
 #include "device_once.cuh"
 #include "gate_math.cuh"
 #include "host_calls.h"
+#include "tc05.cuh"
 
 namespace b200wkv {
 namespace {
@@ -186,11 +187,6 @@ template <typename T, int VEC, int K, bool kWhole> struct Lane {
             }
         }
     }
-    __device__ __forceinline__ void load(P* to, const T* row) const {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (there[k]) to[k].load(row + k * step, second[k]);
-    }
     __device__ __forceinline__ void store(T* row, int k, const F2* v) const { P::store(row + k * step, v, second[k]); }
     // x less its mean over the team (0 where there is nothing), and 1 / sqrt(var + eps)
     template <bool kBlock> __device__ __forceinline__ float centre(F2 (&x)[K][kPairs], const Problem& p, float inv_d, float* room) const {
@@ -215,6 +211,55 @@ template <typename T, int VEC, int K, bool kWhole> struct Lane {
         return rsqrtf(team_sum<kBlock>(sum_of(sums), p.team, room) * inv_d + p.eps);
     }
 };
+// A stream's pieces of the rows to come.  kAsync: pieces of 16 bytes travel to shared memory by cp.async, three rows in front of the one at
+// work (two of two pieces each); the registers would hold one row, a third of what keeps the memory busy.  A thread reads only
+// what it has asked for itself, so no barrier is needed.  Else one row ahead, in registers.
+template <typename T, int VEC, int K, bool kWhole, bool kAsync> struct Rows {
+    typedef Lane<T, VEC, K, kWhole> L;
+    static constexpr int kAhead = !kAsync ? 1 : K == 1 ? 3 : 2;
+    static constexpr size_t kBytes = kAsync ? (size_t)kAhead * K * 16 : 0;     // a thread's of shared memory
+    const T* from;                         // the thread's first piece of the row to ask for next
+    long long step;                        // elements to the row after it
+    unsigned char* room;
+    typename L::P q[K];
+    __device__ __forceinline__ Rows(const void* p, long long stride, const Problem& pr, const Place& at, const L& my, int which, unsigned char* shared)
+        : from((const T*)p + at.first * stride + my.c), step(pr.parallel * stride), room(shared + ((size_t)which * kAhead * K * blockDim.x + threadIdx.x) * 16), q{} {}
+    __device__ __forceinline__ unsigned char* slot(int place, int k) const { return room + (size_t)(place * K + k) * blockDim.x * 16; }
+    __device__ __forceinline__ void ask(int place, bool on, const L& my) {
+        if (on) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (my.there[k]) {
+                    if constexpr (kAsync) tc::cp_async16(slot(place, k), from + k * my.step, true);
+                    else q[k].load(from + k * my.step, my.second[k]);
+                }
+        }
+        from += step;
+    }
+    __device__ __forceinline__ void take(int place, F2 (&v)[K][L::kPairs], const L& my) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if constexpr (kAsync) {
+                q[k] = typename L::P{};
+                if (my.there[k]) q[k].load((const T*)slot(place, k), true);
+            }
+            q[k].unpack(v[k]);
+        }
+    }
+};
+// Where that pays.  32768 rows of 32 groups of 64, bf16, gated: forward 80 -> 76 us, backward 136 -> 122; 8190 rows of 8 groups of 512 (two pieces
+// a thread): forward 51 -> 47, backward 79 -> 83 without a gate, 87 -> 87 with one; in fp32, where a piece is half as many numbers for the same
+// instructions, backward 115 -> 134; whole CTAs a group: forward 51 -> 53, backward 103 -> 108.
+template <typename T, int K, bool kWhole, bool kBlock, bool kForward> constexpr bool kAsyncRows = sizeof(T) == 2 && kWhole && !kBlock && (kForward || K == 1);
+
+// the row at work has arrived; those behind it may be on their way
+template <int kAhead, bool kAsync> __device__ __forceinline__ void asked() {
+    if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kAhead, bool kAsync> __device__ __forceinline__ void arrived() {
+    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+}
+
 template <typename Go> __device__ __forceinline__ void by_activation(int act, Go go) {
     if (act == B200WKV_ACT_SILU) go(std::integral_constant<int, B200WKV_ACT_SILU>());
     else if (act == B200WKV_ACT_SIGMOID) go(std::integral_constant<int, B200WKV_ACT_SIGMOID>());
@@ -226,37 +271,35 @@ constexpr int fwd_ctas(int elements, int bytes, bool gate) { return elements <= 
 __host__ __device__ constexpr int bwd_ctas(int elements) { return elements <= 4 ? 3 : elements <= 8 ? 2 : 1; }
 
 template <typename T, int VEC, int K, bool kWhole, bool kBlock, bool kGate>
-__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : fwd_ctas(VEC * K, kWhole ? VEC * K * (int)sizeof(T) : 32, kGate))
+__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock && VEC * K <= 8 ? 2 : kBlock ? 1 : fwd_ctas(VEC * K, kWhole ? VEC * K * (int)sizeof(T) : 32, kGate))
 group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
     typedef Lane<T, VEC, K, kWhole> L;
     __shared__ float room[kBlock ? 32 : 1];
     const Place at(p);
     const L my(p, at);
     const float inv_d = 1.f / (float)p.D;
-    typename L::P rx[K] = {}, rg[K] = {};
-    const T* px = (const T*)p.x + at.first * p.x_stride + my.c;
-    const T* pg = kGate ? (const T*)p.gate + at.first * p.gate_stride + my.c : nullptr;
-    T* py = y + at.first * p.C + my.c;
-    const auto read = [&](long long row) {
-        if (row < p.rows) {
-            my.load(rx, px);
-            if (kGate) my.load(rg, pg);
-        }
-        px += p.parallel * p.x_stride;
-        if (kGate) pg += p.parallel * p.gate_stride;
+    extern __shared__ __align__(16) unsigned char shared[];
+    constexpr bool kAsync = VEC == 8 && kAsyncRows<T, K, kWhole, kBlock, true>;
+    typedef Rows<T, VEC, K, kWhole, kAsync> R;
+    R rx(p.x, p.x_stride, p, at, my, 0, shared), rg(p.gate, p.gate_stride, p, at, my, 1, shared);
+    const auto ask = [&](int place, long long row) {
+        rx.ask(place, row < p.rows, my);
+        if (kGate) rg.ask(place, row < p.rows, my);
+        asked<R::kAhead, kAsync>();
     };
-    read(at.first);
+    for (int i = 0; i < R::kAhead; ++i) ask(i, at.first + (long long)i * p.parallel);
+    T* py = y + at.first * p.C + my.c;
     // (teams without work go along: the sums take whole warps and CTAs)
     const long long steps = (p.rows + p.parallel - 1) / p.parallel;
     long long row = at.first;
+    int place = 0;
     for (long long i = 0; i < steps; ++i, row += p.parallel, py += (long long)p.parallel * p.C) {
         F2 x[K][L::kPairs], g[K][L::kPairs];
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            rx[k].unpack(x[k]);
-            if (kGate) rg[k].unpack(g[k]);
-        }
-        read(row + p.parallel);
+        arrived<R::kAhead, kAsync>();
+        rx.take(place, x, my);
+        if (kGate) rg.take(place, g, my);
+        ask(place, row + (long long)R::kAhead * p.parallel);
+        place = place + 1 == R::kAhead ? 0 : place + 1;
         const F2 rstd = both(my.template centre<kBlock>(x, p, inv_d, room));
         by_activation(p.act, [&](auto act) {
 #pragma unroll
@@ -282,7 +325,6 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     typedef Lane<T, VEC, K, kWhole> L;
     constexpr int kPairs = L::kPairs;
     __shared__ float room[kBlock ? 32 : 1];
-    __shared__ float both_sums[kBlock ? 1 : 2 * 256 * VEC];
     const Place at(p);
     const L my(p, at);
     const float inv_d = 1.f / (float)p.D;
@@ -291,34 +333,30 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) dw[k][i] = db[k][i] = both(0.f);
-    typename L::P rx[K] = {}, rg[K] = {}, rd[K] = {};
-    const T* px = (const T*)p.x + at.first * p.x_stride + my.c;
-    const T* pg = kGate ? (const T*)p.gate + at.first * p.gate_stride + my.c : nullptr;
-    const T* pd = gy + at.first * p.C + my.c;
-    long long dense = at.first * p.C + my.c;
-    const auto read = [&](long long row) {
-        if (row < p.rows) {
-            my.load(rx, px);
-            my.load(rd, pd);
-            if (kGate) my.load(rg, pg);
-        }
-        px += p.parallel * p.x_stride;
-        pd += (long long)p.parallel * p.C;
-        if (kGate) pg += p.parallel * p.gate_stride;
+    extern __shared__ __align__(16) unsigned char shared[];
+    constexpr bool kAsync = VEC == 8 && kAsyncRows<T, K, kWhole, kBlock, false>;
+    typedef Rows<T, VEC, K, kWhole, kAsync> R;
+    R rx(p.x, p.x_stride, p, at, my, 0, shared), rd(gy, p.C, p, at, my, 1, shared), rg(p.gate, p.gate_stride, p, at, my, 2, shared);
+    const auto ask = [&](int place, long long row) {
+        rx.ask(place, row < p.rows, my);
+        rd.ask(place, row < p.rows, my);
+        if (kGate) rg.ask(place, row < p.rows, my);
+        asked<R::kAhead, kAsync>();
     };
-    read(at.first);
+    for (int i = 0; i < R::kAhead; ++i) ask(i, at.first + (long long)i * p.parallel);
+    long long dense = at.first * p.C + my.c;
     const long long steps = (p.rows + p.parallel - 1) / p.parallel;
     long long row = at.first;
+    int place = 0;
     for (long long i = 0; i < steps; ++i, row += p.parallel, dense += (long long)p.parallel * p.C) {
         const bool on = row < p.rows;
         F2 x[K][kPairs], g[K][kPairs], d[K][kPairs];
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            rx[k].unpack(x[k]);
-            rd[k].unpack(d[k]);
-            if (kGate) rg[k].unpack(g[k]);
-        }
-        read(row + p.parallel);
+        arrived<R::kAhead, kAsync>();
+        rx.take(place, x, my);
+        rd.take(place, d, my);
+        if (kGate) rg.take(place, g, my);
+        ask(place, row + (long long)R::kAhead * p.parallel);
+        place = place + 1 == R::kAhead ? 0 : place + 1;
         const F2 rstd = both(my.template centre<kBlock>(x, p, inv_d, room));
         F2 s1 = both(0.f), s2 = both(0.f);                // of dxh and dxh xh
         by_activation(p.act, [&](auto act) {
@@ -357,6 +395,7 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     // partial rows (parallel or one per CTA, 2, C): weight, bias
     const auto of = [](const F2* v, int i) { return i % 2 == 0 ? parts(v[i / 2]).x : parts(v[i / 2]).y; };
     if (!kBlock && p.reduce) {             // teams of one group within the CTA are added first, a column a thread
+        float* const both_sums = (float*)shared;             // (every copy into it has arrived)
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             __syncthreads();
@@ -446,6 +485,10 @@ Plan plan_of(Problem& p, int element, int aligned, bool forward) {
     const int threads = forward ? 2048 : 256 * bwd_ctas(q.vec * q.k) < 512 ? 512 : 256 * bwd_ctas(q.vec * q.k), ctas = threads > q.block ? threads / q.block : 1;
     const long long most_ctas = (long long)sm_count_of_current_device() * (ctas < 32 ? ctas : 32);
     long long grid = (all + p.per_cta - 1) / p.per_cta;
+    if (!forward) {                        // four rows a team before there is a second CTA on an SM: each more is a partial row to add
+        const long long four = (grid + 3) / 4, one = sm_count_of_current_device();
+        grid = grid < one ? grid : four < one ? one : four;
+    }
     grid = grid < most_ctas ? grid : most_ctas;
     if (p.reduce) {
         grid = grid < kMaxPartials ? grid : kMaxPartials;
@@ -465,6 +508,11 @@ int aligned_to(std::initializer_list<const void*> ps, std::initializer_list<long
     for (const void* q : ps) bits |= reinterpret_cast<uintptr_t>(q);
     for (long long s : strides) bits |= (uintptr_t)s * element;
     return (int)(bits & (0 - bits));
+}
+// Shared memory of a CTA: the rows to come of so many streams, and behind them the CTA's sums of the parameters' gradients.
+template <typename T, int VEC, int K, bool kWhole, bool kAsync> size_t shared_bytes(const Plan& q, int streams, bool sums) {
+    const size_t rows = Rows<T, VEC, K, kWhole, kAsync>::kBytes * streams * q.block, room = sums ? 2 * 256 * VEC * sizeof(float) : 0;
+    return rows > room ? rows : room;
 }
 // `go` for the cut of a plan
 template <typename T, typename Go> int dispatch(const Plan& q, const Problem& p, Go go) {
@@ -494,7 +542,10 @@ template <typename T, typename Go> int dispatch(const Plan& q, const Problem& p,
 template <typename T> int fwd(cudaStream_t st, Problem p, void* y) {
     const Plan q = plan_of(p, sizeof(T), aligned_to({p.x, p.gate, y}, {p.x_stride, p.gate_stride, p.C}, sizeof(T)), true);
     return dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto gate) {
-        group_norm_fwd_kernel<T, vec.value, k.value, whole.value, block.value, gate.value><<<q.grid, q.block, 0, st>>>(p, (T*)y);
+        const auto kern = group_norm_fwd_kernel<T, vec.value, k.value, whole.value, block.value, gate.value>;
+        constexpr bool kAsync = vec.value == 8 && kAsyncRows<T, k.value, whole.value, block.value, true>;
+        const size_t smem = shared_bytes<T, vec.value, k.value, whole.value, kAsync>(q, 1 + gate.value, false);       // (48 KB at most)
+        kern<<<q.grid, q.block, smem, st>>>(p, (T*)y);
         return cudaGetLastError() == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
     });
 }
@@ -504,8 +555,10 @@ int bwd(cudaStream_t st, Problem p, const void* gy, void* dx, void* dgate, void*
     const bool params = dweight != nullptr || dbias != nullptr;
     if (!params) partial = nullptr;
     const int status = dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto gate) {
-        group_norm_bwd_kernel<T, vec.value, k.value, whole.value, block.value, gate.value>
-            <<<q.grid, q.block, 0, st>>>(p, (const T*)gy, (T*)dx, (T*)dgate, partial);
+        const auto kern = group_norm_bwd_kernel<T, vec.value, k.value, whole.value, block.value, gate.value>;
+        constexpr bool kAsync = vec.value == 8 && kAsyncRows<T, k.value, whole.value, block.value, false>;
+        const size_t smem = shared_bytes<T, vec.value, k.value, whole.value, kAsync>(q, 2 + gate.value, p.reduce);    // (36 KB at most)
+        kern<<<q.grid, q.block, smem, st>>>(p, (const T*)gy, (T*)dx, (T*)dgate, partial);
         return cudaGetLastError() == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
     });
     if (status != B200WKV_OK || !params) return status;

@@ -136,14 +136,14 @@ template <typename T, int kAct> __device__ __forceinline__ void activate(F2 z, F
     dp = kAct == B200WKV_ACT_SIGMOID ? mul2(s, r) : mul2(s, fma2(z, r, both(1.f)));
 }
 
-// sum over the team, the same in every thread of it
+// sum over the team, the same in every thread of it.  Whole CTAs: a row's sums have places of their own in `room`, so that one barrier
+// each is enough (a place is written again behind the barrier of the next sum, which everyone reaches after reading it).
 template <bool kBlock> __device__ __forceinline__ float team_sum(float a, int team, float* room) {
 #pragma unroll
     for (int o = 16; o > 0; o /= 2)
         if (kBlock || team > o) a += __shfl_xor_sync(0xffffffffu, a, o);
     if (kBlock) {
         const int warps = blockDim.x / 32;
-        __syncthreads();                   // the last sums have been read
         if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = a;
         __syncthreads();
         a = 0.f;
@@ -208,7 +208,7 @@ template <typename T, int VEC, int K, bool kWhole> struct Lane {
             }
             if (there[k]) sums = add2(sums, squares);
         }
-        return rsqrtf(team_sum<kBlock>(sum_of(sums), p.team, room) * inv_d + p.eps);
+        return rsqrtf(team_sum<kBlock>(sum_of(sums), p.team, room + kMaxThreads / 32) * inv_d + p.eps);
     }
 };
 // A stream's pieces of the rows to come.  kAsync: pieces of 16 bytes travel to shared memory by cp.async, three rows in front of the one at
@@ -268,13 +268,13 @@ template <typename Go> __device__ __forceinline__ void by_activation(int act, Go
 
 // CTAs of 256 threads an SM for the registers of a kernel: weight, bias, a row's values and the next row's as they lie in memory
 constexpr int fwd_ctas(int elements, int bytes, bool gate) { return elements <= 4 || (elements <= 8 && bytes <= 16) ? 4 : elements <= 8 || !gate ? 3 : 2; }
-__host__ __device__ constexpr int bwd_ctas(int elements) { return elements <= 4 ? 3 : elements <= 8 ? 2 : 1; }
+__host__ __device__ constexpr int bwd_ctas(int elements, bool gate) { return elements <= 4 ? 3 : elements <= 8 || !gate ? 2 : 1; }
 
 template <typename T, int VEC, int K, bool kWhole, bool kBlock, bool kGate>
 __global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock && VEC * K <= 8 ? 2 : kBlock ? 1 : fwd_ctas(VEC * K, kWhole ? VEC * K * (int)sizeof(T) : 32, kGate))
 group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
     typedef Lane<T, VEC, K, kWhole> L;
-    __shared__ float room[kBlock ? 32 : 1];
+    __shared__ float room[kBlock ? 4 * kMaxThreads / 32 : 1];
     const Place at(p);
     const L my(p, at);
     const float inv_d = 1.f / (float)p.D;
@@ -320,11 +320,11 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
 }
 
 template <typename T, int VEC, int K, bool kWhole, bool kBlock, bool kGate>
-__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : bwd_ctas(VEC * K))
+__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : bwd_ctas(VEC * K, kGate))
 group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ partial) {
     typedef Lane<T, VEC, K, kWhole> L;
     constexpr int kPairs = L::kPairs;
-    __shared__ float room[kBlock ? 32 : 1];
+    __shared__ float room[kBlock ? 4 * kMaxThreads / 32 : 1];
     const Place at(p);
     const L my(p, at);
     const float inv_d = 1.f / (float)p.D;
@@ -381,7 +381,8 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
                 }
             }
         });
-        const F2 m1 = both(-team_sum<kBlock>(sum_of(s1), p.team, room) * inv_d), m2 = both(-team_sum<kBlock>(sum_of(s2), p.team, room) * inv_d);
+        const F2 m1 = both(-team_sum<kBlock>(sum_of(s1), p.team, room + 2 * kMaxThreads / 32) * inv_d);
+        const F2 m2 = both(-team_sum<kBlock>(sum_of(s2), p.team, room + 3 * kMaxThreads / 32) * inv_d);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (!my.there[k] || !on) continue;
@@ -482,7 +483,7 @@ Plan plan_of(Problem& p, int element, int aligned, bool forward) {
     p.per_cta = p.reduce ? teams / p.G * p.G : teams;
     const long long all = p.rows * p.G;                  // rows of groups
     // as many threads as the device has room for: a backward keeps its parameters' sums, so its CTAs are no more than are resident
-    const int threads = forward ? 2048 : 256 * bwd_ctas(q.vec * q.k) < 512 ? 512 : 256 * bwd_ctas(q.vec * q.k), ctas = threads > q.block ? threads / q.block : 1;
+    const int threads = forward ? 2048 : q.vec * q.k <= 4 ? 768 : 512, ctas = threads > q.block ? threads / q.block : 1;
     const long long most_ctas = (long long)sm_count_of_current_device() * (ctas < 32 ? ctas : 32);
     long long grid = (all + p.per_cta - 1) / p.per_cta;
     if (!forward) {                        // four rows a team before there is a second CTA on an SM: each more is a partial row to add

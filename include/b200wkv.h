@@ -51,7 +51,7 @@ const char* b200wkv_strerror(int status);
 int b200wkv_abi_version(void);
 /* Diagnostics: reads and clears the device-side error word of the current device (0 = none).
  * The tensor-core kernels bound every wait on an asynchronous product; a wait that runs out is
- * recorded there (1 = forward, 2 = backward) and the kernel still terminates.  This call
+ * recorded there (1 = forward, 2 = backward, 3 = gated recurrence) and the kernel still terminates.  This call
  * synchronises the device, so it is not for the hot path.  Returns -1 if the CUDA runtime fails. */
 int b200wkv_device_status(void);
 
@@ -238,8 +238,8 @@ int b200wkv7_mix_post_bwd(void* stream, int dtype, long long rows, int H, int N,
  * computed for all T tokens.  A start flag drops the state in front of its token whatever it holds.  length NULL: T
  * everywhere; new_starts NULL: none; s0 NULL: zeros.
  *
- * `residual` (b200wkv_gated_residual_bytes) is filled by the forward for the backward, which only reads it; NULL for
- * inference.  gy or gs may be NULL (= zeros).  No output may overlap an input. */
+ * `residual` (b200wkv_gated_residual_bytes, 16-byte aligned) is filled by the forward for the backward, which only reads it;
+ * NULL for inference.  gy or gs may be NULL (= zeros).  No output may overlap an input. */
 #define B200WKV_GATE_SIGMOID 0
 #define B200WKV_GATE_DECAY   1
 size_t b200wkv_gated_residual_bytes(int B, int T, int C);

@@ -571,7 +571,7 @@ int b200wkv_gated_fwd(void* stream, int dtype, int gate, int B, int T, int C, co
     if (st != B200WKV_OK) return st;
     if (!x || !f || !y || !s_out) return B200WKV_ENULL;
     if (residual != nullptr && residual_bytes < gated_residual_bytes(B, T, C)) return B200WKV_ERESIDUAL;
-    if (!aligned(element_bytes(dtype), {x, f, y}) || !aligned(4, {s0, length, s_out, residual})) return B200WKV_EUNSUPPORTED;
+    if (!aligned(element_bytes(dtype), {x, f, y}) || !aligned(4, {s0, length, s_out}) || !aligned(16, {residual})) return B200WKV_EUNSUPPORTED;
     if (T == 1 && residual == nullptr && s0 != nullptr)
         return gated_step((cudaStream_t)stream, dtype, gate, B, C, x, x_batch, f, f_batch, s0, C, length, new_starts, y, s_out, C);
     return gated_fwd((cudaStream_t)stream, dtype, gate, B, T, C, x, x_batch, x_token, f, f_batch, f_token, s0, length, new_starts, y, s_out,
@@ -585,7 +585,7 @@ int b200wkv_gated_bwd(void* stream, int dtype, int gate, int B, int T, int C, co
     if (st != B200WKV_OK) return st;
     if (!x || !f || !residual || !dx || !df || !ds0) return B200WKV_ENULL;
     if (residual_bytes < gated_residual_bytes(B, T, C)) return B200WKV_ERESIDUAL;
-    if (!aligned(element_bytes(dtype), {x, f, gy, dx, df}) || !aligned(4, {gs, length, residual, ds0})) return B200WKV_EUNSUPPORTED;
+    if (!aligned(element_bytes(dtype), {x, f, gy, dx, df}) || !aligned(4, {gs, length, ds0}) || !aligned(16, {residual})) return B200WKV_EUNSUPPORTED;
     return gated_bwd((cudaStream_t)stream, dtype, gate, B, T, C, x, x_batch, x_token, f, f_batch, f_token, length, new_starts, gy, gs, residual,
                      dx, df, ds0);
 }

@@ -22,6 +22,7 @@
 #include <limits.h>
 
 #include <initializer_list>
+#include <type_traits>
 
 #include "common.cuh"
 #include "device_once.cuh"
@@ -36,7 +37,7 @@ using namespace tc;
 
 constexpr int kWarps = 8;
 constexpr int kWide = 64;                  // channels of a CTA
-constexpr int kKept = 64;                  // tokens per kept state, and of a backward tile
+constexpr int kKept = 8;                   // tokens per kept state, and of a backward segment
 constexpr int kMaxCluster = 8;
 constexpr int kStages = 2;
 constexpr int kWaitRanOut = 3;             // status word: a wait for the other CTAs of a cluster
@@ -155,11 +156,19 @@ template <typename T, int kPiece> __device__ __forceinline__ void put(T* p, F2 a
         if (channels > 1) p[1] = from_f32<T>(q.y);
     }
 }
-__device__ __forceinline__ F2 get_state(const float* p, int channels) { return make_f2(p != nullptr ? p[0] : 0.f, p != nullptr && channels > 1 ? p[1] : 0.f); }
-__device__ __forceinline__ void put_state(float* p, F2 h, int channels) {
-    const float2 q = parts(h);
-    p[0] = q.x;
-    if (channels > 1) p[1] = q.y;
+// kPair: both at once, where C is even and the array begins on 8 bytes
+template <bool kPair = false> __device__ __forceinline__ F2 get_state(const float* p, int channels) {
+    if (kPair) return *reinterpret_cast<const F2*>(p);
+    return make_f2(p != nullptr ? p[0] : 0.f, p != nullptr && channels > 1 ? p[1] : 0.f);
+}
+template <bool kPair = false> __device__ __forceinline__ void put_state(float* p, F2 h, int channels) {
+    if (kPair) {
+        *reinterpret_cast<F2*>(p) = h;
+    } else {
+        const float2 q = parts(h);
+        p[0] = q.x;
+        if (channels > 1) p[1] = q.y;
+    }
 }
 
 // start flags of the kSeg tokens from t0 on as a bit mask (bit i = token t0 + i)
@@ -179,7 +188,7 @@ struct Exchange {
             mbar_init(&bar[1], 1);
             mbar_init_fence();
         }
-        if (ranks > 1) cluster_sync();
+        cluster_sync();
     }
     __device__ __forceinline__ void send(int round, int rank, int ranks, const Stretch& tile, int lane) {   // by one warp
         uint64_t* const mine = &bar[round & 1];
@@ -193,7 +202,7 @@ struct Exchange {
         if (status != nullptr) *status = kWaitRanOut;
     }
     // no CTA leaves while others may still send to it
-    __device__ __forceinline__ void close(int ranks) { if (ranks > 1) cluster_sync(); }
+    __device__ __forceinline__ void close() { cluster_sync(); }
 };
 
 // Grid: x the 64 channels and, inside, the CTAs of a cluster; y and z the sequence
@@ -243,20 +252,45 @@ struct Chain {
     }
 };
 
-template <typename T> constexpr int kFwdSeg = sizeof(T) == 2 ? 16 : 8;
-constexpr int kBwdSeg = kKept / kWarps;
+// How the state goes from warp to warp where one CTA has the sequence: in turn, each with its segment.  A warp's box is written again
+// when its last content has gone around through all of them.
+struct Mail {
+    F2 box[kWarps][32];
+    uint64_t bar[kWarps];
+    __device__ __forceinline__ void open() {
+        if (threadIdx.x == 0)
+            for (int w = 0; w < kWarps; ++w) mbar_init(&bar[w], 1);
+        __syncthreads();
+    }
+    __device__ __forceinline__ F2 take(int warp, int phase, bool& lost, int* status) {
+        if (!lost && !mbar_wait(&bar[warp], phase & 1)) {
+            lost = true;
+            if (status != nullptr) *status = kWaitRanOut;
+        }
+        return box[warp][threadIdx.x & 31];
+    }
+    __device__ __forceinline__ void pass(int to, F2 h) {
+        box[to][threadIdx.x & 31] = h;
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&bar[to]);
+    }
+};
 
-template <typename T, int kGate, int kPiece>
+template <typename T> constexpr int kFwdSeg = sizeof(T) == 2 ? 16 : 8;
+constexpr int kBwdSeg = kKept;
+
+// kTurn: one CTA has the sequence, and its warps take the state over from one another, so that nothing is summarised and no barrier
+// joins them.  Else a cluster shares it.
+template <typename T, int kGate, int kPiece, bool kTurn>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, float* __restrict__ kept) {
     constexpr int kSeg = kFwdSeg<T>, kTile = kSeg * kWarps, kRow = kWide * (int)sizeof(T), kRoom = 2 * kSeg * kRow;
     extern __shared__ __align__(128) unsigned char dynamic[];
-    __shared__ Exchange ex;
-    __shared__ Chain chain[2];
-    __shared__ F2 carried[2][32];
+    __shared__ std::conditional_t<kTurn, Mail, Exchange> ex;
+    __shared__ std::conditional_t<kTurn, char, Chain> chain[2];
     const Place at(p);
     if (at.bi >= p.B) return;              // (a whole cluster)
-    const int lane = at.lane, warp = at.warp, ranks = at.ranks, c0 = at.c0;
+    const int lane = at.lane, warp = at.warp, rank = kTurn ? 0 : at.rank, ranks = kTurn ? 1 : at.ranks, c0 = at.c0;
     const size_t state = at.state(p);
     const int tiles = (p.T + kTile - 1) / kTile, rounds = (tiles + ranks - 1) / ranks;
     const Feed<T, kPiece, kSeg> fx(p.x.p, p.x.batch, p.x.token, at.bi, c0, p.C), ff(p.f.p, p.f.batch, p.f.token, at.bi, c0, p.C);
@@ -264,26 +298,30 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
     const auto ask = [&](int round) {
         if (round < rounds) {
             const uint32_t to = smem_u32(room) + round % kStages * kRoom;
-            fx.fetch(to, (round * ranks + at.rank) * kTile, p.T);
-            ff.fetch(to + kSeg * kRow, (round * ranks + at.rank) * kTile, p.T);
+            fx.fetch(to, (round * ranks + rank) * kTile, p.T);
+            ff.fetch(to + kSeg * kRow, (round * ranks + rank) * kTile, p.T);
         }
         fetched();
     };
     for (int i = 0; i < kStages; ++i) ask(i);
-    F2 carry = get_state(p.s0 != nullptr ? p.s0 + state : nullptr, at.channels);      // state entering the round
-    if (at.L == 0 && warp == 0 && at.rank == 0) put_state(s_out + state, carry, at.channels);
-    if (warp == kWarps - 1) carried[0][lane] = carry;
-    chain[0].pad();
-    chain[1].pad();
-    ex.open(ranks);
+    F2 carry = get_state(p.s0 != nullptr ? p.s0 + state : nullptr, at.channels);      // state entering the round (kTurn: the sequence)
+    if (at.L == 0 && warp == 0 && rank == 0) put_state(s_out + state, carry, at.channels);
+    if constexpr (kTurn) {
+        ex.open();
+    } else {
+        chain[0].pad();
+        chain[1].pad();
+        ex.open(ranks);
+    }
     bool lost = false;
     const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)at.bi * p.T : nullptr;
     const uint32_t down = p.C * (uint32_t)sizeof(T), own_off = warp * kSeg * down + at.col * (uint32_t)sizeof(T);
+    const int states = (p.T + kKept - 1) / kKept;
     for (int round = 0; round < rounds; ++round) {
-        const int tile = (round * ranks + at.rank) * kTile, t0 = tile + warp * kSeg, n = max(0, min(kSeg, p.T - t0)), parity = round & 1;
+        const int tile = (round * ranks + rank) * kTile, t0 = tile + warp * kSeg, n = max(0, min(kSeg, p.T - t0));
         const uint32_t starts = segment_flags<kSeg>(ns, t0, p.T, lane);
         const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
-        // 1. gates and increments, and what the segment does
+        // 1. gates and increments
         F2 a[kSeg], u[kSeg];
         wait_fetched<kStages - 1>();
         const T* const from = (const T*)(room + round % kStages * kRoom) + at.col;
@@ -296,112 +334,118 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
         }
         __syncwarp();                      // the segment has been read
         ask(round + kStages);
-        F2 A = both(1.f), b = both(0.f);
-        const auto summarise = [&](auto kind) {
-#pragma unroll
-            for (int i = 0; i < kSeg; ++i) {
-                if (!kind.value) {
-                    if (i >= n) { a[i] = both(1.f); u[i] = both(0.f); }
-                    if ((starts >> i) & 1u) { A = both(-1.f); b = u[i]; continue; }
-                }
-                b = fma2(a[i], b, u[i]);
-                A = mul2(A, a[i]);
-            }
-        };
-        if (plain) summarise(Plain()); else summarise(Marked());
-        chain[parity].of(warp) = Stretch{A, b};
-        const bool marked = __syncthreads_or(starts != 0);       // a start flag in the tile
-        // 2. the state that enters the tile, and the one that enters the segment
+        // 2. the state that enters the segment
         F2 h;
-        if (ranks > 1) {
-            if (warp == kWarps - 1) ex.send(round, at.rank, ranks, chain[parity].all(), lane);
+        if constexpr (kTurn) {
+            h = warp == 0 && round == 0 ? carry : ex.take(warp, warp == 0 ? round - 1 : round, lost, p.status);
+        } else {
+            const int parity = round & 1;
+            F2 A = both(1.f), b = both(0.f);
+            const auto summarise = [&](auto kind) {
+#pragma unroll
+                for (int i = 0; i < kSeg; ++i) {
+                    if (!kind.value) {
+                        if (i >= n) { a[i] = both(1.f); u[i] = both(0.f); }
+                        if ((starts >> i) & 1u) { A = both(-1.f); b = u[i]; continue; }
+                    }
+                    b = fma2(a[i], b, u[i]);
+                    A = mul2(A, a[i]);
+                }
+            };
+            if (plain) summarise(Plain()); else summarise(Marked());
+            chain[parity].of(warp) = Stretch{A, b};
+            const bool marked = __syncthreads_or(starts != 0);   // a start flag in the tile
+            if (warp == kWarps - 1) ex.send(round, rank, ranks, chain[parity].all(), lane);
             ex.wait(round, lost, p.status);
             for (int q = 0; q < ranks; ++q) {
-                if (q == at.rank) h = carry;
+                if (q == rank) h = carry;
                 carry = ex.tiles[parity][q][lane].of(carry);
             }
-        } else {
-            h = carried[parity][lane];
+            h = chain[parity].follow(h, warp, marked);
         }
-        h = chain[parity].follow(h, warp, marked);
-        // (a kept state is wanted in front of every 64th token; the returned one behind its token)
-        if (kept != nullptr && n > 0 && t0 % kKept == 0) put_state(kept + ((size_t)at.bi * ((p.T + kKept - 1) / kKept) + t0 / kKept) * p.C + c0 + at.col, h, at.channels);
-        // 3. outputs
+        // 3. the states; outputs, and the states that are kept
         char* const to = (char*)y + (((long long)at.bi * p.T + tile) * p.C + c0) * (long long)sizeof(T);
+        const F2 first = h;
         const auto walk = [&](auto kind) {
+#pragma unroll
+            for (int i = 0; i < kSeg; ++i) {
+                const bool start = !kind.value && ((starts >> i) & 1u);
+                if (kind.value || i < n) u[i] = h = start ? u[i] : fma2(a[i], h, u[i]);
+            }
+            if constexpr (kTurn) ex.pass((warp + 1) % kWarps, h);
             uint32_t off = own_off;
 #pragma unroll
             for (int i = 0; i < kSeg; ++i, off += down) {
-                const bool start = !kind.value && ((starts >> i) & 1u);
-                h = start ? u[i] : fma2(a[i], h, u[i]);
-                if (kind.value || i < n) put<T, kPiece>((T*)(to + off), h, at.channels);
-                if (!kind.value && t0 + i == at.L - 1) put_state(s_out + state, h, at.channels);
+                if (kind.value || i < n) {
+                    put<T, kPiece>((T*)(to + off), u[i], at.channels);
+                    if (kept != nullptr && i % kKept == 0)
+                        put_state<(kPiece > 4)>(kept + ((long long)at.bi * states + t0 / kKept + i / kKept) * p.C + c0 + at.col, i == 0 ? first : u[i == 0 ? 0 : i - 1], at.channels);
+                }
+                if (!kind.value && t0 + i == at.L - 1) put_state(s_out + state, u[i], at.channels);
             }
         };
         if (plain) walk(Plain()); else walk(Marked());
-        if (ranks == 1 && warp == kWarps - 1) carried[parity ^ 1][lane] = h;
     }
-    ex.close(ranks);
+    if constexpr (!kTurn) ex.close();
 }
 
-template <typename T, int kGate, int kPiece>
+template <typename T, int kGate, int kPiece, bool kTurn>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restrict__ gs, const float* __restrict__ kept,
                  T* __restrict__ dx, T* __restrict__ df, float* __restrict__ ds0) {
-    constexpr int kSeg = kBwdSeg, kTile = kKept, kRow = kWide * (int)sizeof(T), kRoom = 3 * kSeg * kRow;
+    constexpr int kSeg = kBwdSeg, kTile = kSeg * kWarps, kRow = kWide * (int)sizeof(T), kRoom = 3 * kSeg * kRow;
     extern __shared__ __align__(128) unsigned char dynamic[];
-    __shared__ Exchange ex;
-    __shared__ Chain chain[2], back[2];
-    __shared__ F2 carried[2][32];
+    __shared__ std::conditional_t<kTurn, Mail, Exchange> ex;
+    __shared__ std::conditional_t<kTurn, char, Chain> back[2];
     const Place at(p);
     if (at.bi >= p.B) return;              // (a whole cluster)
-    const int lane = at.lane, warp = at.warp, ranks = at.ranks, c0 = at.c0;
+    const int lane = at.lane, warp = at.warp, rank = kTurn ? 0 : at.rank, ranks = kTurn ? 1 : at.ranks, c0 = at.c0;
     const size_t state = at.state(p);
-    const int tiles = (p.T + kTile - 1) / kTile, rounds = (tiles + ranks - 1) / ranks;
+    const int tiles = (p.T + kTile - 1) / kTile, rounds = (tiles + ranks - 1) / ranks, states = (p.T + kKept - 1) / kKept;
     const Feed<T, kPiece, kSeg> fx(p.x.p, p.x.batch, p.x.token, at.bi, c0, p.C), ff(p.f.p, p.f.batch, p.f.token, at.bi, c0, p.C);
     const Feed<T, kPiece, kSeg> fg(gy, (long long)p.T * p.C, p.C, at.bi, c0, p.C);
     unsigned char* const room = dynamic + warp * kStages * kRoom;
-    // rounds are taken from the last to the first
-    const auto stage = [&](int round) { return (rounds - 1 - round) % kStages * kRoom; };
-    const auto ask = [&](int round) {
-        if (round >= 0) {
-            const uint32_t to = smem_u32(room) + stage(round);
-            const int tile = (round * ranks + at.rank) * kTile;
+    // rounds are taken from the last to the first; `done` of them lie behind
+    const auto ask = [&](int done) {
+        if (done < rounds) {
+            const uint32_t to = smem_u32(room) + done % kStages * kRoom;
+            const int tile = ((rounds - 1 - done) * ranks + rank) * kTile;
             fx.fetch(to, tile, p.T);
             ff.fetch(to + kSeg * kRow, tile, p.T);
             if (gy != nullptr) fg.fetch(to + 2 * kSeg * kRow, tile, p.T);
         }
         fetched();
     };
-    const auto entering = [&](int round) { // the kept state in front of a round's tile
-        const int tile = round * ranks + at.rank;
-        return round >= 0 && tile < tiles ? get_state(kept + ((long long)at.bi * tiles + tile) * p.C + c0 + at.col, at.channels) : both(0.f);
+    const auto entering = [&](int done) {  // the kept state in front of the warp's segment
+        const int seg = ((rounds - 1 - done) * ranks + rank) * kWarps + warp;
+        return done < rounds && seg < states ? get_state<(kPiece > 4)>(kept + ((long long)at.bi * states + seg) * p.C + c0 + at.col, at.channels) : both(0.f);
     };
     if (gy == nullptr)                     // nothing is fetched there, and zeros are read
         for (int i = 0; i < kStages; ++i)
             for (int j = lane; j < kSeg * kRow / 4; j += 32) ((uint32_t*)(room + i * kRoom + 2 * kSeg * kRow))[j] = 0;
-    for (int i = 0; i < kStages; ++i) ask(rounds - 1 - i);
-    F2 next = entering(rounds - 1), carry = both(0.f);       // carry: c entering the round from behind
+    for (int i = 0; i < kStages; ++i) ask(i);
+    F2 next = entering(0), carry = both(0.f);                    // carry: c entering the round from behind
     const F2 gstate = get_state(gs != nullptr ? gs + state : nullptr, at.channels);
-    if (warp == 0) carried[(rounds - 1) & 1][lane] = carry;
-    chain[0].pad();
-    chain[1].pad();
-    back[0].pad();
-    back[1].pad();
-    ex.open(ranks);
+    if constexpr (kTurn) {
+        ex.open();
+    } else {
+        back[0].pad();
+        back[1].pad();
+        ex.open(ranks);
+    }
     bool lost = false;
     const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)at.bi * p.T : nullptr;
-    const uint32_t down = p.C * (uint32_t)sizeof(T), own_off = (warp * kSeg + kSeg - 1) * down + at.col * (uint32_t)sizeof(T);
-    for (int round = rounds - 1; round >= 0; --round) {
-        const int tile = (round * ranks + at.rank) * kTile, t0 = tile + warp * kSeg, n = max(0, min(kSeg, p.T - t0)), parity = round & 1;
+    const uint32_t down = p.C * (uint32_t)sizeof(T), own_off = warp * kSeg * down + at.col * (uint32_t)sizeof(T);
+    for (int done = 0; done < rounds; ++done) {
+        const int tile = ((rounds - 1 - done) * ranks + rank) * kTile, t0 = tile + warp * kSeg, n = max(0, min(kSeg, p.T - t0));
         const uint32_t starts = segment_flags<kSeg>(ns, t0, p.T, lane);
         const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
         F2 h = next;
-        next = entering(round - 1);
-        // 1. gates; what the segment does to the states, and what it sends to the front
+        next = entering(done + 1);
+        // 1. gates, states, and in the place of x what df is dx times of
         F2 a[kSeg], w[kSeg], x[kSeg], g[kSeg];
         wait_fetched<kStages - 1>();
-        const T* const from = (const T*)(room + stage(round)) + at.col;
+        const T* const from = (const T*)(room + done % kStages * kRoom) + at.col;
 #pragma unroll
         for (int i = 0; i < kSeg; ++i) {
             x[i] = pair_at(from + i * kWide);
@@ -409,69 +453,72 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
             g[i] = pair_at(from + (2 * kSeg + i) * kWide);
         }
         __syncwarp();                      // the segment has been read
-        ask(round - kStages);
-        const auto increment = [&](int i) { return kGate == kSigmoidGate ? mul2(w[i], x[i]) : x[i]; };
-        F2 A = both(1.f), b = both(0.f), c = both(0.f);
-        const auto summarise = [&](auto kind) {
+        ask(done + kStages);
+        const auto replay = [&](auto kind) {
 #pragma unroll
             for (int i = 0; i < kSeg; ++i) {
                 if (!kind.value) {
                     if (i >= n) { a[i] = both(1.f); w[i] = x[i] = both(0.f); }
                     if (t0 + i == at.L - 1) g[i] = add2(g[i], gstate);
-                    if ((starts >> i) & 1u) { A = both(-1.f); b = increment(i); continue; }
                 }
-                b = fma2(a[i], b, increment(i));
-                A = mul2(A, a[i]);
-            }
-#pragma unroll
-            for (int i = kSeg - 1; i >= 0; --i) c = !kind.value && ((starts >> i) & 1u) ? both(0.f) : mul2(a[i], add2(g[i], c));
-        };
-        if (plain) summarise(Plain()); else summarise(Marked());
-        chain[parity].of(warp) = Stretch{A, b};
-        back[parity].of(kWarps - 1 - warp) = Stretch{A, c};
-        const bool marked = __syncthreads_or(starts != 0);       // a start flag in the tile
-        // 2. the state that enters the segment, and c that enters it from behind
-        F2 e;
-        if (ranks > 1) {
-            if (warp == 0) ex.send(rounds - 1 - round, at.rank, ranks, back[parity].all(), lane);
-            ex.wait(rounds - 1 - round, lost, p.status);
-            for (int q = ranks - 1; q >= 0; --q) {
-                if (q == at.rank) e = carry;
-                carry = ex.tiles[(rounds - 1 - round) & 1][q][lane].of(carry);
-            }
-        } else {
-            e = carried[parity][lane];
-        }
-        h = chain[parity].follow(h, warp, marked);
-        e = back[parity].follow(e, kWarps - 1 - warp, marked);
-        // 3. the states again, and in the place of x what df is dx times of; then back through the segment
-        const long long tile_at = (((long long)at.bi * p.T + tile) * p.C + c0) * (long long)sizeof(T);
-        char *const to_x = (char*)dx + tile_at, *const to_f = (char*)df + tile_at;
-        const auto walk = [&](auto kind) {
-#pragma unroll
-            for (int i = 0; i < kSeg; ++i) {
                 const bool start = !kind.value && ((starts >> i) & 1u);
-                const F2 in = start ? both(0.f) : h, u = increment(i);
+                const F2 in = start ? both(0.f) : h, u = kGate == kSigmoidGate ? mul2(w[i], x[i]) : x[i];
                 h = start ? u : fma2(a[i], h, u);
                 if (kGate == kSigmoidGate) x[i] = mul2(fma2(x[i], both(-1.f), in), a[i]);
                 else x[i] = start ? both(0.f) : mul2(mul2(in, w[i]), both(-1.f));
             }
+        };
+        if (plain) replay(Plain()); else replay(Marked());
+        // 2. what comes to the segment from behind
+        F2 e;
+        if constexpr (kTurn) {
+            e = done == 0 && warp == kWarps - 1 ? carry : ex.take(warp, warp == kWarps - 1 ? done - 1 : done, lost, p.status);
+        } else {
+            const int parity = done & 1;
+            F2 A = both(1.f), c = both(0.f);
+            const auto summarise = [&](auto kind) {
+#pragma unroll
+                for (int i = kSeg - 1; i >= 0; --i) {
+                    const bool start = !kind.value && ((starts >> i) & 1u);
+                    A = start ? both(-1.f) : mul2(A, a[i]);
+                    c = start ? both(0.f) : mul2(a[i], add2(g[i], c));
+                }
+            };
+            if (plain) summarise(Plain()); else summarise(Marked());
+            back[parity].of(kWarps - 1 - warp) = Stretch{A, c};
+            const bool marked = __syncthreads_or(starts != 0);   // a start flag in the tile
+            if (warp == 0) ex.send(done, rank, ranks, back[parity].all(), lane);
+            ex.wait(done, lost, p.status);
+            for (int q = ranks - 1; q >= 0; --q) {
+                if (q == rank) e = carry;
+                carry = ex.tiles[parity][q][lane].of(carry);
+            }
+            e = back[parity].follow(e, kWarps - 1 - warp, marked);
+        }
+        // 3. back through the segment
+        const long long tile_at = (((long long)at.bi * p.T + tile) * p.C + c0) * (long long)sizeof(T);
+        char *const to_x = (char*)dx + tile_at, *const to_f = (char*)df + tile_at;
+        const auto walk = [&](auto kind) {
+#pragma unroll
+            for (int i = kSeg - 1; i >= 0; --i) {
+                g[i] = add2(g[i], e);
+                e = !kind.value && ((starts >> i) & 1u) ? both(0.f) : mul2(a[i], g[i]);
+            }
+            if constexpr (kTurn) ex.pass((warp + kWarps - 1) % kWarps, e);
             uint32_t off = own_off;
 #pragma unroll
-            for (int i = kSeg - 1; i >= 0; --i, off -= down) {
-                const F2 d = add2(g[i], e), o = kGate == kSigmoidGate ? mul2(d, w[i]) : d, of = mul2(o, x[i]);
+            for (int i = 0; i < kSeg; ++i, off += down) {
+                const F2 o = kGate == kSigmoidGate ? mul2(g[i], w[i]) : g[i], of = mul2(o, x[i]);
                 if (kind.value || i < n) {
                     put<T, kPiece>((T*)(to_x + off), o, at.channels);
                     put<T, kPiece>((T*)(to_f + off), of, at.channels);
                 }
-                e = !kind.value && ((starts >> i) & 1u) ? both(0.f) : mul2(a[i], d);
             }
         };
         if (plain) walk(Plain()); else walk(Marked());
         if (t0 == 0) put_state(ds0 + state, at.L == 0 ? add2(e, gstate) : e, at.channels);
-        if (ranks == 1 && warp == 0) carried[parity ^ 1][lane] = e;
     }
-    ex.close(ranks);
+    if constexpr (!kTurn) ex.close();
 }
 
 // One token: out = h = (start ? 0 : a s) + u; rows of length 0 keep their state (and have their output all the same).  A thread's
@@ -511,12 +558,12 @@ gated_step_kernel(int B, int C, const T* x, long long x_stride, const T* f, long
 struct Residency {
     DeviceOnce once;
     int clusters[kMaxDevices][kMaxCluster + 1];
-    template <typename Kernel> const int* of(Kernel kern, size_t smem) {
+    template <typename Kernel> const int* of(Kernel kern, size_t smem, int largest) {
         const int dev = current_device();
         if (dev < 0) return nullptr;
         const bool ok = once.ok([&]() {
             const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            for (int n = 1; n <= kMaxCluster; ++n) {
+            for (int n = 1; n <= largest; ++n) {
                 cudaLaunchAttribute attr[1];
                 cudaLaunchConfig_t cfg = config(attr, n, dim3(n), smem, nullptr);
                 int fit = 0;
@@ -543,27 +590,29 @@ struct Residency {
         return cfg;
     }
 };
-// CTAs of a cluster: those with which the last sequence is done after the fewest rounds, waves of clusters counted; the smaller of equals.
+// CTAs of a cluster: those with which the last sequence is done soonest, by the rounds that it takes and the waves of clusters in front of it; the
+// smaller of equals.  One CTA alone passes the state from warp to warp and takes kAlone of a cluster's time for a round.
 // units: 64 channels of a sequence each; tiles: of one of them.
-int ranks_of(const int* resident, long long units, int tiles) {
+int ranks_of(const int* alone, const int* resident, long long units, int tiles) {
+    constexpr double kAlone = 0.6;
     int best = 1;
-    long long least = LLONG_MAX;
-    for (int n = 1; n <= kMaxCluster && n <= tiles; ++n) {
+    double least = kAlone * ((units + alone[1] - 1) / alone[1]) * tiles;
+    for (int n = 2; n <= kMaxCluster && n <= tiles; ++n) {
         if (resident[n] < 1) continue;
-        const long long rounds = (units + resident[n] - 1) / resident[n] * ((tiles + n - 1) / n);
+        const double rounds = (double)((units + resident[n] - 1) / resident[n]) * ((tiles + n - 1) / n);
         if (rounds < least) { least = rounds; best = n; }
     }
     return best;
 }
 template <typename Kernel, typename... Args>
-int launch(Residency& residency, Kernel kern, cudaStream_t st, const Problem& p, int tile, size_t smem, Args... args) {
-    const int* const resident = residency.of(kern, smem);
-    if (resident == nullptr) return B200WKV_ELAUNCH;
-    const int slabs = (p.C + kWide - 1) / kWide, ranks = ranks_of(resident, (long long)p.B * slabs, (p.T + tile - 1) / tile);
+int launch(Residency (&residency)[2], Kernel turn, Kernel cluster, cudaStream_t st, const Problem& p, int tile, size_t smem, Args... args) {
+    const int *const alone = residency[0].of(turn, smem, 1), *const resident = residency[1].of(cluster, smem, kMaxCluster);
+    if (alone == nullptr || resident == nullptr || alone[1] < 1) return B200WKV_ELAUNCH;
+    const int slabs = (p.C + kWide - 1) / kWide, ranks = ranks_of(alone, resident, (long long)p.B * slabs, (p.T + tile - 1) / tile);
     const unsigned y = p.B < 65535 ? p.B : 65535;
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg = Residency::config(attr, ranks, dim3((unsigned)slabs * ranks, y, (p.B + y - 1) / y), smem, st);
-    return cudaLaunchKernelEx(&cfg, kern, p, args...) == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
+    return cudaLaunchKernelEx(&cfg, ranks > 1 ? cluster : turn, p, args...) == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
 }
 // The widest pieces that every row of these begins on.
 int piece_of(int C, int element, std::initializer_list<const void*> streams, std::initializer_list<long long> strides) {
@@ -574,14 +623,14 @@ int piece_of(int C, int element, std::initializer_list<const void*> streams, std
 }
 
 template <typename T, int kGate, int kPiece> int fwd(cudaStream_t st, const Problem& p, void* y, float* s_out, float* kept) {
-    static Residency once;
+    static Residency residency[2];
     constexpr int kTile = kFwdSeg<T> * kWarps;
-    return launch(once, gated_fwd_kernel<T, kGate, kPiece>, st, p, kTile, (size_t)kStages * 2 * kTile * kWide * sizeof(T), (T*)y, s_out, kept);
+    return launch(residency, gated_fwd_kernel<T, kGate, kPiece, true>, gated_fwd_kernel<T, kGate, kPiece, false>, st, p, kTile, (size_t)kStages * 2 * kTile * kWide * sizeof(T), (T*)y, s_out, kept);
 }
 template <typename T, int kGate, int kPiece>
 int bwd(cudaStream_t st, const Problem& p, const void* gy, const float* gs, const float* kept, void* dx, void* df, float* ds0) {
-    static Residency once;
-    return launch(once, gated_bwd_kernel<T, kGate, kPiece>, st, p, kKept, (size_t)kStages * 3 * kKept * kWide * sizeof(T), (const T*)gy, gs, kept,
+    static Residency residency[2];
+    return launch(residency, gated_bwd_kernel<T, kGate, kPiece, true>, gated_bwd_kernel<T, kGate, kPiece, false>, st, p, kBwdSeg * kWarps, (size_t)kStages * 3 * kBwdSeg * kWarps * kWide * sizeof(T), (const T*)gy, gs, kept,
                   (T*)dx, (T*)df, ds0);
 }
 // calls `go` with the element type, the gate and the piece as template arguments

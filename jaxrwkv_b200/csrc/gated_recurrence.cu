@@ -591,10 +591,12 @@ struct Residency {
     }
 };
 // CTAs of a cluster: those with which the last sequence is done soonest, by the rounds that it takes and the waves of clusters in front of it; the
-// smaller of equals.  One CTA alone passes the state from warp to warp and takes kAlone of a cluster's time for a round.
+// smaller of equals.  One CTA alone passes the state from warp to warp and takes kAlone of a cluster's time for a round.  Forward / backward in us with
+// one CTA a sequence and with clusters, bf16: B=4, T=1024, C=2048 20 / 29 and 25 / 31 (of two); B=16, T=512, C=768 16 / 22 and 27 / 33 (two); B=2,
+// T=8192, C=1024 98 / 156 and 35 / 51 (eight); B=1, T=2000, C=2560 30 and 21 (six); fp32, B=4, T=2048, C=2048 43 / 64 and 45 / 80 (two).
 // units: 64 channels of a sequence each; tiles: of one of them.
 int ranks_of(const int* alone, const int* resident, long long units, int tiles) {
-    constexpr double kAlone = 0.6;
+    constexpr double kAlone = 0.5;
     int best = 1;
     double least = kAlone * ((units + alone[1] - 1) / alone[1]) * tiles;
     for (int n = 2; n <= kMaxCluster && n <= tiles; ++n) {

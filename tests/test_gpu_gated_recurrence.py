@@ -48,6 +48,27 @@ def test_many_sequences_and_channels(dtype):
 
 
 @pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,C", [(150, 8), (150, 6), (150, 5), (4, 2600)])
+def test_a_thread_block_a_sequence(B, C, dtype, gate):
+    """So many sequences or channels that none is shared: some of them, over several tiles, in pieces of every size."""
+    x, f, s, length, ns, gy, gs = cuda(*inputs(B, 300, C, gate, dtype, seed=C, starts=0.02))
+    got = train(x, f, s, length, ns, gate, gs, gy)
+    for b in (0, B // 2, B - 1):
+        cut, ch = slice(b, b + 1), slice(max(0, C - 40), C)
+        check_gated([t[cut][..., ch] for t in got], x[cut][..., ch], f[cut][..., ch], s[cut][..., ch], length[cut], ns[cut], gate, gs[cut][..., ch],
+                    gy[cut][..., ch])
+
+
+def test_more_sequences_than_a_grid_axis():
+    B = 70001
+    x, f, s, length, ns, gy, gs = cuda(*inputs(B, 2, 2, "sigmoid", torch.bfloat16, seed=3, starts=0.1))
+    got = train(x, f, s, length, ns, "sigmoid", gs, gy)
+    at = [0, 65534, 65535, 65536, B - 1]
+    check_gated([t[at] for t in got], x[at], f[at], s[at], length[at], ns[at], "sigmoid", gs[at], gy[at])
+
+
+@pytest.mark.parametrize("gate", GATES)
 @pytest.mark.parametrize("lengths", [[0, 0, 0], [1, 130, 64], [65, 63, 128], [300, 1000, 129]])
 def test_lengths_and_dense_flags(lengths, gate):
     """The returned state at every kind of place (longer than T is T); flags on almost every token."""
@@ -94,8 +115,9 @@ def test_strided_and_shared_cotangents():
         assert torch.equal(a, b)
 
 
-def test_one_cotangent_alone():
-    x, f, s, length, ns, gy, gs = cuda(*inputs(2, 100, 24, "sigmoid", torch.float32, seed=8, starts=0.02))
+@pytest.mark.parametrize("T", [100, 900])
+def test_one_cotangent_alone(T):
+    x, f, s, length, ns, gy, gs = cuda(*inputs(2, T, 24, "sigmoid", torch.float32, seed=8, starts=0.02))
     for use_state in (False, True):
         leaves = [t.detach().requires_grad_(True) for t in (x, f, s)]
         s_out, out = gated_recurrence(*leaves, length, ns)

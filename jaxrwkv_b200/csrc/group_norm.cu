@@ -138,10 +138,11 @@ template <typename T, int kAct> __device__ __forceinline__ void activate(F2 z, F
 
 // sum over the team, the same in every thread of it.  Whole CTAs: a row's sums have places of their own in `room`, so that one barrier
 // each is enough (a place is written again behind the barrier of the next sum, which everyone reaches after reading it).
-template <bool kBlock> __device__ __forceinline__ float team_sum(float a, int team, float* room) {
+// kTeam: the team's lanes where they are known to the compiler, else 0 (five branches a sum).
+template <bool kBlock, int kTeam> __device__ __forceinline__ float team_sum(float a, int team, float* room) {
 #pragma unroll
     for (int o = 16; o > 0; o /= 2)
-        if (kBlock || team > o) a += __shfl_xor_sync(0xffffffffu, a, o);
+        if (kBlock || (kTeam ? kTeam : team) > o) a += __shfl_xor_sync(0xffffffffu, a, o);
     if (kBlock) {
         const int warps = blockDim.x / 32;
         if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = a;
@@ -154,12 +155,12 @@ template <bool kBlock> __device__ __forceinline__ float team_sum(float a, int te
 
 // Where a thread's team works: group g, rows first, first + parallel, ...; none of them where `at_work` is false
 struct Place {
-    int g, lane;
+    int team, g, lane;
     long long first;
     bool at_work;
-    __device__ __forceinline__ Place(const Problem& p) {
-        const int in_cta = threadIdx.x / p.team, q = blockIdx.x * p.per_cta + in_cta;
-        lane = threadIdx.x % p.team;
+    __device__ __forceinline__ Place(const Problem& p, int team_) : team(team_) {
+        const int in_cta = (int)threadIdx.x / team, q = blockIdx.x * p.per_cta + in_cta;
+        lane = (int)threadIdx.x % team;
         g = q % p.G;
         first = q / p.G;
         at_work = in_cta < p.per_cta && first < p.parallel;
@@ -173,10 +174,10 @@ template <typename T, int VEC, int K, bool kWhole> struct Lane {
     int c, step;                           // the first piece's channel in the row
     bool there[K], second[K];              // the piece; its second element (kWhole false)
     F2 w[K][kPairs], b[K][kPairs];
-    __device__ __forceinline__ Lane(const Problem& p, const Place& at) : c(at.g * p.D + at.lane * VEC), step(p.team * VEC) {
+    __device__ __forceinline__ Lane(const Problem& p, const Place& at) : c(at.g * p.D + at.lane * VEC), step(at.team * VEC) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int d = (at.lane + k * p.team) * VEC;
+            const int d = (at.lane + k * at.team) * VEC;
             there[k] = at.at_work && d < p.D;
             second[k] = kWhole || d + 1 < p.D;
 #pragma unroll
@@ -189,13 +190,13 @@ template <typename T, int VEC, int K, bool kWhole> struct Lane {
     }
     __device__ __forceinline__ void store(T* row, int k, const F2* v) const { P::store(row + k * step, v, second[k]); }
     // x less its mean over the team (0 where there is nothing), and 1 / sqrt(var + eps)
-    template <bool kBlock> __device__ __forceinline__ float centre(F2 (&x)[K][kPairs], const Problem& p, float inv_d, float* room) const {
+    template <bool kBlock, int kTeam> __device__ __forceinline__ float centre(F2 (&x)[K][kPairs], const Problem& p, float inv_d, float* room) const {
         F2 sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) sums = add2(sums, x[k][j]);
-        const F2 less = both(-team_sum<kBlock>(sum_of(sums), p.team, room) * inv_d);
+        const F2 less = both(-team_sum<kBlock, kTeam>(sum_of(sums), p.team, room) * inv_d);
         sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -208,7 +209,7 @@ template <typename T, int VEC, int K, bool kWhole> struct Lane {
             }
             if (there[k]) sums = add2(sums, squares);
         }
-        return rsqrtf(team_sum<kBlock>(sum_of(sums), p.team, room + kMaxThreads / 32) * inv_d + p.eps);
+        return rsqrtf(team_sum<kBlock, kTeam>(sum_of(sums), p.team, room + kMaxThreads / 32) * inv_d + p.eps);
     }
 };
 // A stream's pieces of the rows to come.  kAsync: pieces of 16 bytes travel to shared memory by cp.async, three rows in front of the one at
@@ -270,12 +271,12 @@ template <typename Go> __device__ __forceinline__ void by_activation(int act, Go
 constexpr int fwd_ctas(int elements, int bytes, bool gate) { return elements <= 4 || (elements <= 8 && bytes <= 16) ? 4 : elements <= 8 || !gate ? 3 : 2; }
 __host__ __device__ constexpr int bwd_ctas(int elements, bool gate) { return elements <= 4 ? 3 : elements <= 8 || !gate ? 2 : 1; }
 
-template <typename T, int VEC, int K, bool kWhole, bool kBlock, bool kGate>
+template <typename T, int VEC, int K, bool kWhole, bool kBlock, int kTeam, bool kGate>
 __global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock && VEC * K <= 8 ? 2 : kBlock ? 1 : fwd_ctas(VEC * K, kWhole ? VEC * K * (int)sizeof(T) : 32, kGate))
 group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
     typedef Lane<T, VEC, K, kWhole> L;
     __shared__ float room[kBlock ? 4 * kMaxThreads / 32 : 1];
-    const Place at(p);
+    const Place at(p, kBlock ? (int)blockDim.x : kTeam ? kTeam : p.team);
     const L my(p, at);
     const float inv_d = 1.f / (float)p.D;
     extern __shared__ __align__(16) unsigned char shared[];
@@ -300,7 +301,7 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
         if (kGate) rg.take(place, g, my);
         ask(place, row + (long long)R::kAhead * p.parallel);
         place = place + 1 == R::kAhead ? 0 : place + 1;
-        const F2 rstd = both(my.template centre<kBlock>(x, p, inv_d, room));
+        const F2 rstd = both(my.template centre<kBlock, kTeam>(x, p, inv_d, room));
         by_activation(p.act, [&](auto act) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -319,13 +320,13 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
     }
 }
 
-template <typename T, int VEC, int K, bool kWhole, bool kBlock, bool kGate>
+template <typename T, int VEC, int K, bool kWhole, bool kBlock, int kTeam, bool kGate>
 __global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : bwd_ctas(VEC * K, kGate))
 group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ partial) {
     typedef Lane<T, VEC, K, kWhole> L;
     constexpr int kPairs = L::kPairs;
     __shared__ float room[kBlock ? 4 * kMaxThreads / 32 : 1];
-    const Place at(p);
+    const Place at(p, kBlock ? (int)blockDim.x : kTeam ? kTeam : p.team);
     const L my(p, at);
     const float inv_d = 1.f / (float)p.D;
     F2 dw[K][kPairs], db[K][kPairs];
@@ -357,7 +358,7 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
         if (kGate) rg.take(place, g, my);
         ask(place, row + (long long)R::kAhead * p.parallel);
         place = place + 1 == R::kAhead ? 0 : place + 1;
-        const F2 rstd = both(my.template centre<kBlock>(x, p, inv_d, room));
+        const F2 rstd = both(my.template centre<kBlock, kTeam>(x, p, inv_d, room));
         F2 s1 = both(0.f), s2 = both(0.f);                // of dxh and dxh xh
         by_activation(p.act, [&](auto act) {
 #pragma unroll
@@ -381,8 +382,8 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
                 }
             }
         });
-        const F2 m1 = both(-team_sum<kBlock>(sum_of(s1), p.team, room + 2 * kMaxThreads / 32) * inv_d);
-        const F2 m2 = both(-team_sum<kBlock>(sum_of(s2), p.team, room + 3 * kMaxThreads / 32) * inv_d);
+        const F2 m1 = both(-team_sum<kBlock, kTeam>(sum_of(s1), p.team, room + 2 * kMaxThreads / 32) * inv_d);
+        const F2 m2 = both(-team_sum<kBlock, kTeam>(sum_of(s2), p.team, room + 3 * kMaxThreads / 32) * inv_d);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (!my.there[k] || !on) continue;
@@ -520,30 +521,43 @@ template <typename T, typename Go> int dispatch(const Plan& q, const Problem& p,
     constexpr int kWide = 16 / sizeof(T);
     typedef std::true_type Yes;
     typedef std::false_type No;
-    const auto gated = [&](auto vec, auto k, auto whole, auto block) {
-        return p.gate != nullptr ? go(vec, k, whole, block, Yes()) : go(vec, k, whole, block, No());
-    };
+    typedef std::integral_constant<int, 0> Any;
     typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, 2> Two;
     typedef std::integral_constant<int, 4> Four;
     typedef std::integral_constant<int, 8> Eight;
+    typedef std::integral_constant<int, 16> Sixteen;
+    typedef std::integral_constant<int, 32> Warp;
     typedef std::integral_constant<int, kWide> Wide;
+    const auto gated = [&](auto vec, auto k, auto whole, auto block, auto team) {
+        return p.gate != nullptr ? go(vec, k, whole, block, team, Yes()) : go(vec, k, whole, block, team, No());
+    };
     const bool block = p.team > 32;
     if (q.vec == kWide) {
-        if (!block) return q.k == 1 ? gated(Wide(), One(), Yes(), No()) : gated(Wide(), Two(), Yes(), No());
-        if (q.k == 1) return gated(Wide(), One(), Yes(), Yes());
-        if constexpr (sizeof(T) == 4) {                  // (in 16 bits two pieces a thread cover the widest group)
-            if (q.k == 4) return gated(Wide(), Four(), Yes(), Yes());
+        if (!block) {
+            if (q.k == 2) return gated(Wide(), Two(), Yes(), No(), Warp());    // (more than 32 pieces)
+            return p.team == 32   ? gated(Wide(), One(), Yes(), No(), Warp())
+                   : p.team == 16 ? gated(Wide(), One(), Yes(), No(), Sixteen())
+                   : p.team == 8  ? gated(Wide(), One(), Yes(), No(), Eight())
+                                  : gated(Wide(), One(), Yes(), No(), Any());
         }
-        return gated(Wide(), Two(), Yes(), Yes());
+        if (q.k == 1) return gated(Wide(), One(), Yes(), Yes(), Any());
+        if constexpr (sizeof(T) == 4) {                  // (in 16 bits two pieces a thread cover the widest group)
+            if (q.k == 4) return gated(Wide(), Four(), Yes(), Yes(), Any());
+        }
+        return gated(Wide(), Two(), Yes(), Yes(), Any());
     }
-    if (q.whole) return !block ? gated(Two(), Four(), Yes(), No()) : q.k == 4 ? gated(Two(), Four(), Yes(), Yes()) : gated(Two(), Eight(), Yes(), Yes());
-    return !block ? gated(Two(), Four(), No(), No()) : q.k == 4 ? gated(Two(), Four(), No(), Yes()) : gated(Two(), Eight(), No(), Yes());
+    if (q.whole) {
+        if (!block) return gated(Two(), Four(), Yes(), No(), Any());
+        return q.k == 4 ? gated(Two(), Four(), Yes(), Yes(), Any()) : gated(Two(), Eight(), Yes(), Yes(), Any());
+    }
+    if (!block) return gated(Two(), Four(), No(), No(), Any());
+    return q.k == 4 ? gated(Two(), Four(), No(), Yes(), Any()) : gated(Two(), Eight(), No(), Yes(), Any());
 }
 template <typename T> int fwd(cudaStream_t st, Problem p, void* y) {
     const Plan q = plan_of(p, sizeof(T), aligned_to({p.x, p.gate, y}, {p.x_stride, p.gate_stride, p.C}, sizeof(T)), true);
-    return dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto gate) {
-        const auto kern = group_norm_fwd_kernel<T, vec.value, k.value, whole.value, block.value, gate.value>;
+    return dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto team, auto gate) {
+        const auto kern = group_norm_fwd_kernel<T, vec.value, k.value, whole.value, block.value, team.value, gate.value>;
         constexpr bool kAsync = vec.value == 8 && kAsyncRows<T, k.value, whole.value, block.value, true>;
         const size_t smem = shared_bytes<T, vec.value, k.value, whole.value, kAsync>(q, 1 + gate.value, false);       // (48 KB at most)
         kern<<<q.grid, q.block, smem, st>>>(p, (T*)y);
@@ -555,8 +569,8 @@ int bwd(cudaStream_t st, Problem p, const void* gy, void* dx, void* dgate, void*
     const Plan q = plan_of(p, sizeof(T), aligned_to({p.x, p.gate, gy, dx, dgate}, {p.x_stride, p.gate_stride, p.C}, sizeof(T)), false);
     const bool params = dweight != nullptr || dbias != nullptr;
     if (!params) partial = nullptr;
-    const int status = dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto gate) {
-        const auto kern = group_norm_bwd_kernel<T, vec.value, k.value, whole.value, block.value, gate.value>;
+    const int status = dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto team, auto gate) {
+        const auto kern = group_norm_bwd_kernel<T, vec.value, k.value, whole.value, block.value, team.value, gate.value>;
         constexpr bool kAsync = vec.value == 8 && kAsyncRows<T, k.value, whole.value, block.value, false>;
         const size_t smem = shared_bytes<T, vec.value, k.value, whole.value, kAsync>(q, 2 + gate.value, p.reduce);    // (36 KB at most)
         kern<<<q.grid, q.block, smem, st>>>(p, (const T*)gy, (T*)dx, (T*)dgate, partial);

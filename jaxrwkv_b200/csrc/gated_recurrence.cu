@@ -233,21 +233,23 @@ struct Chain {
         for (int i = threadIdx.x; i < (kWarps - 1) * 32; i += kWarps * 32) s[i / 32][i % 32] = Stretch::nothing();
     }
     __device__ __forceinline__ Stretch& of(int place) { return s[kWarps - 1 + place][threadIdx.x & 31]; }
-    // the state that enters the first segment, as it enters the one at `place`
-    __device__ __forceinline__ F2 follow(F2 h, int place, bool marked) const {
+    // the stretch in front of the segment at `place`: of the identities and all segments in front of it
+    __device__ __forceinline__ Stretch front(int place, bool marked) const {
         const Stretch(*const q)[32] = &s[place];
+        return joined(q, kWarps - 1, marked);
+    }
+    __device__ __forceinline__ Stretch all(bool marked) const { return joined(&s[kWarps - 1], kWarps, marked); }
+    __device__ __forceinline__ static Stretch joined(const Stretch (*q)[32], int n, bool marked) {
+        Stretch t = q[0][threadIdx.x & 31];
         if (!marked) {
 #pragma unroll
-            for (int j = 0; j < kWarps - 1; ++j) h = q[j][threadIdx.x & 31].of_uncut(h);
+            for (int j = 1; j < n; ++j) {
+                const Stretch next = q[j][threadIdx.x & 31];
+                t = {mul2(t.A, next.A), next.of_uncut(t.b)};
+            }
         } else {
-            for (int j = 0; j < kWarps - 1; ++j) h = q[j][threadIdx.x & 31].of(h);
+            for (int j = 1; j < n; ++j) t = t.then(q[j][threadIdx.x & 31]);
         }
-        return h;
-    }
-    __device__ __forceinline__ Stretch all() {
-        Stretch t = of(0);
-#pragma unroll
-        for (int j = 1; j < kWarps; ++j) t = t.then(of(j));
         return t;
     }
 };
@@ -355,13 +357,16 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
             if (plain) summarise(Plain()); else summarise(Marked());
             chain[parity].of(warp) = Stretch{A, b};
             const bool marked = __syncthreads_or(starts != 0);   // a start flag in the tile
-            if (warp == kWarps - 1) ex.send(round, rank, ranks, chain[parity].all(), lane);
+            if (warp == kWarps - 1) ex.send(round, rank, ranks, chain[parity].all(marked), lane);
+            const Stretch front = chain[parity].front(warp, marked);
             ex.wait(round, lost, p.status);
-            for (int q = 0; q < ranks; ++q) {
+#pragma unroll
+            for (int q = 0; q < kMaxCluster; ++q) {
+                if (q >= ranks) break;
                 if (q == rank) h = carry;
                 carry = ex.tiles[parity][q][lane].of(carry);
             }
-            h = chain[parity].follow(h, warp, marked);
+            h = front.of(h);
         }
         // 3. the states; outputs, and the states that are kept
         char* const to = (char*)y + (((long long)at.bi * p.T + tile) * p.C + c0) * (long long)sizeof(T);
@@ -487,13 +492,16 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
             if (plain) summarise(Plain()); else summarise(Marked());
             back[parity].of(kWarps - 1 - warp) = Stretch{A, c};
             const bool marked = __syncthreads_or(starts != 0);   // a start flag in the tile
-            if (warp == 0) ex.send(done, rank, ranks, back[parity].all(), lane);
+            if (warp == 0) ex.send(done, rank, ranks, back[parity].all(marked), lane);
+            const Stretch rear = back[parity].front(kWarps - 1 - warp, marked);
             ex.wait(done, lost, p.status);
-            for (int q = ranks - 1; q >= 0; --q) {
+#pragma unroll
+            for (int q = kMaxCluster - 1; q >= 0; --q) {
+                if (q >= ranks) continue;
                 if (q == rank) e = carry;
                 carry = ex.tiles[parity][q][lane].of(carry);
             }
-            e = back[parity].follow(e, kWarps - 1 - warp, marked);
+            e = rear.of(e);
         }
         // 3. back through the segment
         const long long tile_at = (((long long)at.bi * p.T + tile) * p.C + c0) * (long long)sizeof(T);
@@ -593,10 +601,12 @@ struct Residency {
 // CTAs of a cluster: those with which the last sequence is done soonest, by the rounds that it takes and the waves of clusters in front of it; the
 // smaller of equals.  One CTA alone passes the state from warp to warp and takes kAlone of a cluster's time for a round.  Forward / backward in us with
 // one CTA a sequence and with clusters, bf16: B=4, T=1024, C=2048 20 / 29 and 25 / 31 (of two); B=16, T=512, C=768 16 / 22 and 27 / 33 (two); B=2,
-// T=8192, C=1024 98 / 156 and 35 / 51 (eight); B=1, T=2000, C=2560 30 and 21 (six); fp32, B=4, T=2048, C=2048 43 / 64 and 45 / 80 (two).
+// T=8192, C=1024 98 / 156 and 35 / 51 (eight); B=1, T=2000, C=2560 30 and 21 (six); fp32, B=4, T=2048, C=2048 43 / 64 and 45 / 80 (two).  Narrow pieces take a warp longer to ask for:
+// fp32, B=3, T=1023, C=1001 31 / 57 and 23 / 35; bf16, B=4, T=2048, C=1001 92 / 139 and 37 / 57.  (`wide` goes by the row's length alone, so that
+// results do not depend on where operands lie.)
 // units: 64 channels of a sequence each; tiles: of one of them.
-int ranks_of(const int* alone, const int* resident, long long units, int tiles) {
-    constexpr double kAlone = 0.5;
+int ranks_of(const int* alone, const int* resident, long long units, int tiles, bool wide) {
+    const double kAlone = wide ? 0.5 : 0.8;
     int best = 1;
     double least = kAlone * ((units + alone[1] - 1) / alone[1]) * tiles;
     for (int n = 2; n <= kMaxCluster && n <= tiles; ++n) {
@@ -607,10 +617,10 @@ int ranks_of(const int* alone, const int* resident, long long units, int tiles) 
     return best;
 }
 template <typename Kernel, typename... Args>
-int launch(Residency (&residency)[2], Kernel turn, Kernel cluster, cudaStream_t st, const Problem& p, int tile, size_t smem, Args... args) {
+int launch(Residency (&residency)[2], int row_bytes, Kernel turn, Kernel cluster, cudaStream_t st, const Problem& p, int tile, size_t smem, Args... args) {
     const int *const alone = residency[0].of(turn, smem, 1), *const resident = residency[1].of(cluster, smem, kMaxCluster);
     if (alone == nullptr || resident == nullptr || alone[1] < 1) return B200WKV_ELAUNCH;
-    const int slabs = (p.C + kWide - 1) / kWide, ranks = ranks_of(alone, resident, (long long)p.B * slabs, (p.T + tile - 1) / tile);
+    const int slabs = (p.C + kWide - 1) / kWide, ranks = ranks_of(alone, resident, (long long)p.B * slabs, (p.T + tile - 1) / tile, row_bytes % 16 == 0);
     const unsigned y = p.B < 65535 ? p.B : 65535;
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg = Residency::config(attr, ranks, dim3((unsigned)slabs * ranks, y, (p.B + y - 1) / y), smem, st);
@@ -627,12 +637,12 @@ int piece_of(int C, int element, std::initializer_list<const void*> streams, std
 template <typename T, int kGate, int kPiece> int fwd(cudaStream_t st, const Problem& p, void* y, float* s_out, float* kept) {
     static Residency residency[2];
     constexpr int kTile = kFwdSeg<T> * kWarps;
-    return launch(residency, gated_fwd_kernel<T, kGate, kPiece, true>, gated_fwd_kernel<T, kGate, kPiece, false>, st, p, kTile, (size_t)kStages * 2 * kTile * kWide * sizeof(T), (T*)y, s_out, kept);
+    return launch(residency, p.C * (int)sizeof(T), gated_fwd_kernel<T, kGate, kPiece, true>, gated_fwd_kernel<T, kGate, kPiece, false>, st, p, kTile, (size_t)kStages * 2 * kTile * kWide * sizeof(T), (T*)y, s_out, kept);
 }
 template <typename T, int kGate, int kPiece>
 int bwd(cudaStream_t st, const Problem& p, const void* gy, const float* gs, const float* kept, void* dx, void* df, float* ds0) {
     static Residency residency[2];
-    return launch(residency, gated_bwd_kernel<T, kGate, kPiece, true>, gated_bwd_kernel<T, kGate, kPiece, false>, st, p, kBwdSeg * kWarps, (size_t)kStages * 3 * kBwdSeg * kWarps * kWide * sizeof(T), (const T*)gy, gs, kept,
+    return launch(residency, p.C * (int)sizeof(T), gated_bwd_kernel<T, kGate, kPiece, true>, gated_bwd_kernel<T, kGate, kPiece, false>, st, p, kBwdSeg * kWarps, (size_t)kStages * 3 * kBwdSeg * kWarps * kWide * sizeof(T), (const T*)gy, gs, kept,
                   (T*)dx, (T*)df, ds0);
 }
 // calls `go` with the element type, the gate and the piece as template arguments

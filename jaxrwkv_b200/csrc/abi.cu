@@ -551,6 +551,11 @@ int b200wkv_token_shift_bwd(void* stream, int dtype, int B, int T, int D, int M,
 
 static bool known(int dtype) { return dtype == B200WKV_F32 || dtype == B200WKV_BF16; }
 static size_t element_bytes(int dtype) { return dtype == B200WKV_F32 ? 4 : 2; }
+static bool negative(std::initializer_list<long long> strides) {
+    for (long long s : strides)
+        if (s < 0) return true;
+    return false;
+}
 
 // The tiles of a sequence are counted and the grid is made in 32 bits, and so are offsets inside a tile of 128 tokens.
 static int check_gated(int dtype, int gate, int B, int T, int C) {
@@ -569,6 +574,7 @@ int b200wkv_gated_fwd(void* stream, int dtype, int gate, int B, int T, int C, co
                       const uint8_t* new_starts, void* y, float* s_out, void* residual, size_t residual_bytes) {
     int st = check_gated(dtype, gate, B, T, C);
     if (st != B200WKV_OK) return st;
+    if (negative({x_batch, x_token, f_batch, f_token})) return B200WKV_ESHAPE;
     if (!x || !f || !y || !s_out) return B200WKV_ENULL;
     if (residual != nullptr && residual_bytes < gated_residual_bytes(B, T, C)) return B200WKV_ERESIDUAL;
     if (!aligned(element_bytes(dtype), {x, f, y}) || !aligned(4, {s0, length, s_out}) || !aligned(16, {residual})) return B200WKV_EUNSUPPORTED;
@@ -583,6 +589,7 @@ int b200wkv_gated_bwd(void* stream, int dtype, int gate, int B, int T, int C, co
                       const void* gy, const float* gs, const void* residual, size_t residual_bytes, void* dx, void* df, float* ds0) {
     int st = check_gated(dtype, gate, B, T, C);
     if (st != B200WKV_OK) return st;
+    if (negative({x_batch, x_token, f_batch, f_token})) return B200WKV_ESHAPE;
     if (!x || !f || !residual || !dx || !df || !ds0) return B200WKV_ENULL;
     if (residual_bytes < gated_residual_bytes(B, T, C)) return B200WKV_ERESIDUAL;
     if (!aligned(element_bytes(dtype), {x, f, gy, dx, df}) || !aligned(4, {gs, length, ds0}) || !aligned(16, {residual})) return B200WKV_EUNSUPPORTED;
@@ -595,6 +602,7 @@ int b200wkv_gated_step(void* stream, int dtype, int gate, int B, int C, const vo
                        float* s_out, long long s_out_stride) {
     int st = check_gated(dtype, gate, B, 1, C);
     if (st != B200WKV_OK) return st;
+    if (negative({x_stride, f_stride, s_stride, s_out_stride})) return B200WKV_ESHAPE;
     if (!x || !f || !s || !y || !s_out) return B200WKV_ENULL;
     if (!aligned(element_bytes(dtype), {x, f, y}) || !aligned(4, {s, length, s_out})) return B200WKV_EUNSUPPORTED;
     return gated_step((cudaStream_t)stream, dtype, gate, B, C, x, x_stride, f, f_stride, s, s_stride, length, new_starts, y, s_out, s_out_stride);
@@ -612,6 +620,7 @@ int b200wkv_group_norm_fwd(void* stream, int dtype, long long rows, int C, int g
                            long long gate_stride, void* y) {
     int st = check_norm(dtype, rows, C, groups, activation, param_dtype);
     if (st != B200WKV_OK) return st;
+    if (negative({x_stride, gate_stride})) return B200WKV_ESHAPE;
     if (!x || !y) return B200WKV_ENULL;
     if (!aligned(element_bytes(dtype), {x, gate, y}) || !aligned(element_bytes(param_dtype), {weight, bias})) return B200WKV_EUNSUPPORTED;
     return group_norm_fwd((cudaStream_t)stream, dtype, rows, C, groups, eps, activation, x, x_stride, weight, bias, param_dtype, gate,
@@ -628,6 +637,7 @@ int b200wkv_group_norm_bwd(void* stream, int dtype, long long rows, int C, int g
                            size_t workspace_bytes) {
     int st = check_norm(dtype, rows, C, groups, activation, param_dtype);
     if (st != B200WKV_OK) return st;
+    if (negative({x_stride, gate_stride})) return B200WKV_ESHAPE;
     if (!x || !gy || !dx || (gate == nullptr) != (dgate == nullptr)) return B200WKV_ENULL;
     if (dweight != nullptr || dbias != nullptr) {
         if (!workspace) return B200WKV_ENULL;

@@ -958,7 +958,7 @@ std::pair<Tensor, Tensor> gated_step(int64_t gate, const Tensor* t, const Tensor
     check(b200wkv_gated_step(stream_of(x), dtype_code(x), (int)gate, (int)B, (int)C, in(x), x.stride(0), in(f), f.stride(0), (const float*)in(from),
                              from.stride(0), (const uint32_t*)in(len), (const uint8_t*)in(ns), out(y), (float*)out(s_out),
                              in_place ? from.stride(0) : C));
-    if (in_place) torch::autograd::impl::bump_version(s);
+    if (in_place && !s.is_inference()) torch::autograd::impl::bump_version(s);
     return {s_out, y};
 }
 

@@ -194,6 +194,6 @@ def gated_recurrence_step(x, f, s, new_starts=None, length=None, gate="sigmoid",
         length, new_starts = _flag_bytes(length, new_starts, lead, (), x.device)
         _lib.check(lib.b200wkv_gated_step(_stream(), dtype, code, B, C, _ptr(xr), xr.stride(0), _ptr(fr), fr.stride(0), _ptr(sr), sr.stride(0),
                                           _ptr(length), _ptr(new_starts), _ptr(out), _ptr(s_out), sr.stride(0) if inplace else C))
-    if inplace:
+    if inplace and not s.is_inference():
         torch.autograd.graph.increment_version(s)
     return s_out, out

@@ -31,6 +31,7 @@ def test_recurrence_forward(lib):
     for name in ("x", "f", "y", "s_out"):
         assert fwd(lib, **{name: None}) == -3, name
         assert fwd(lib, **{name: ODD}) == -6, name
+    assert lib.b200wkv_gated_fwd(None, 1, 0, 1, 4, 8, A, 32, 8, A, 32, -8, A, None, None, A, A, None, 0) == -2
     assert fwd(lib, s0=ODD) == -6 and fwd(lib, length=P((1 << 12) + 2)) == -6
     assert fwd(lib, residual=A, nbytes=lib.b200wkv_gated_residual_bytes(1, 4, 8) - 1) == -4
 
@@ -58,6 +59,7 @@ def test_group_norm(lib):
     assert norm(dtype=3) == -1 and norm(pd=3) == -1 and norm(act=3) == -6 and norm(act=-1) == -6
     for bad in (dict(rows=0), dict(C=0), dict(G=0), dict(G=5), dict(C=16386, G=2), dict(rows=1 << 31), dict(C=(1 << 24) + 4)):
         assert norm(**bad) == -2, bad
+    assert lib.b200wkv_group_norm_fwd(None, 1, 4, 64, 4, 1e-5, 2, A, -64, A, A, 1, None, 64, A) == -2
     assert norm(x=None) == -3 and norm(y=None) == -3 and norm(x=ODD) == -6 and norm(w=ODD) == -6 and norm(gate=ODD) == -6
 
     need = lib.b200wkv_group_norm_workspace_bytes(4, 64)

@@ -279,6 +279,34 @@ def test_steps_continue_a_sequence(gate):
     check_gated((state, torch.cat(outs, 1)), x, f, s, length, ns, gate)
 
 
+def test_inference_mode():
+    """Tensors without a version counter, the state updated where it lies."""
+    with torch.inference_mode():
+        x, f, s, length, ns, _, _ = cuda(*inputs(2, 70, 48, "sigmoid", torch.bfloat16, seed=19))
+        state, out = gated_recurrence(x, f, s, length, ns)
+        check_gated((state, out), x, f, s, length, ns, "sigmoid")
+        same, o = gated_recurrence_step(x[:, 0], f[:, 0], state, inplace=True)
+        assert same is state
+
+
+def test_two_calls_at_once():
+    """On two streams, many times over: nothing is shared between calls."""
+    sets = [cuda(*inputs(3, 700, 96, "sigmoid", torch.bfloat16, seed=22 + i, starts=0.02)) for i in range(2)]
+    run = lambda q: train(q[0], q[1], q[2], q[3], q[4], "sigmoid", q[6], q[5])
+    want = [run(q) for q in sets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for q, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(run(q))
+        torch.cuda.synchronize()
+        for one, ref in zip(got, want):
+            for a, b in zip(one, ref):
+                assert torch.equal(a, b)
+
+
 def test_another_stream_and_captured_calls():
     """On a side stream; forward and backward captured and replayed on new values, two graphs that take turns."""
     make = lambda seed: cuda(*inputs(2, 150, 64, "sigmoid", torch.bfloat16, seed=seed, starts=0.02))

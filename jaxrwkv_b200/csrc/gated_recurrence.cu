@@ -171,10 +171,10 @@ template <bool kPair = false> __device__ __forceinline__ void put_state(float* p
     }
 }
 
-// start flags of the kSeg tokens from t0 on as a bit mask (bit i = token t0 + i)
-template <int kSeg> __device__ __forceinline__ uint32_t segment_flags(const uint8_t* ns, int t0, int Tlen, int lane) {
-    if (ns == nullptr) return 0;
-    return __ballot_sync(0xffffffffu, lane < kSeg && t0 + lane < Tlen && ns[t0 + lane] != 0);
+// Whether the lane's token of a segment has a start flag; read well before the segment's mask (bit i = token t0 + i) is made of it.
+template <int kSeg> __device__ __forceinline__ bool start_flag(const uint8_t* ns, int t0, int T) {
+    const int lane = threadIdx.x & 31;
+    return ns != nullptr && lane < kSeg && t0 + lane < T && ns[t0 + lane] != 0;
 }
 
 // What the CTAs of a cluster tell one another: the stretches of a round's tiles.  Two rounds' worth: a CTA sends a round's only when
@@ -321,8 +321,7 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
     const int states = (p.T + kKept - 1) / kKept;
     for (int round = 0; round < rounds; ++round) {
         const int tile = (round * ranks + rank) * kTile, t0 = tile + warp * kSeg, n = max(0, min(kSeg, p.T - t0));
-        const uint32_t starts = segment_flags<kSeg>(ns, t0, p.T, lane);
-        const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
+        const bool flag = start_flag<kSeg>(ns, t0, p.T);
         // 1. gates and increments
         F2 a[kSeg], u[kSeg];
         wait_fetched<kStages - 1>();
@@ -336,6 +335,8 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
         }
         __syncwarp();                      // the segment has been read
         ask(round + kStages);
+        const uint32_t starts = __ballot_sync(0xffffffffu, flag);
+        const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
         // 2. the state that enters the segment
         F2 h;
         if constexpr (kTurn) {
@@ -443,7 +444,8 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
     const uint32_t down = p.C * (uint32_t)sizeof(T), own_off = warp * kSeg * down + at.col * (uint32_t)sizeof(T);
     for (int done = 0; done < rounds; ++done) {
         const int tile = ((rounds - 1 - done) * ranks + rank) * kTile, t0 = tile + warp * kSeg, n = max(0, min(kSeg, p.T - t0));
-        const uint32_t starts = segment_flags<kSeg>(ns, t0, p.T, lane);
+        // (asked for behind the gates, as the forward does, the mask costs the registers that the gates are short of: 129 -> 148 us)
+        const uint32_t starts = __ballot_sync(0xffffffffu, start_flag<kSeg>(ns, t0, p.T));
         const bool plain = n == kSeg && starts == 0 && (at.L <= t0 || at.L > t0 + kSeg);
         F2 h = next;
         next = entering(done + 1);

@@ -182,7 +182,7 @@ template <int kSeg> __device__ __forceinline__ bool start_flag(const uint8_t* ns
 struct Exchange {
     Stretch tiles[2][kMaxCluster][32];
     uint64_t bar[2];
-    __device__ __forceinline__ void open(int ranks) {
+    __device__ __forceinline__ void open() {
         if (threadIdx.x == 0) {
             mbar_init(&bar[0], 1);
             mbar_init(&bar[1], 1);
@@ -225,30 +225,22 @@ struct Place {
 struct Plain { static constexpr bool value = true; };      // a whole segment without a start flag in which the returned state is not taken
 struct Marked { static constexpr bool value = false; };
 
-// The segments of a tile by what they do to a state, in the order in which it meets them, behind as many identities as there are
-// segments in front of the last one: every warp goes over seven.
+// The segments of a tile by what they do to a state, in the order in which it meets them.
 struct Chain {
-    Stretch s[kWarps - 1 + kWarps][32];
-    __device__ __forceinline__ void pad() {
-        for (int i = threadIdx.x; i < (kWarps - 1) * 32; i += kWarps * 32) s[i / 32][i % 32] = Stretch::nothing();
-    }
-    __device__ __forceinline__ Stretch& of(int place) { return s[kWarps - 1 + place][threadIdx.x & 31]; }
-    // the stretch in front of the segment at `place`: of the identities and all segments in front of it
-    __device__ __forceinline__ Stretch front(int place, bool marked) const {
-        const Stretch(*const q)[32] = &s[place];
-        return joined(q, kWarps - 1, marked);
-    }
-    __device__ __forceinline__ Stretch all(bool marked) const { return joined(&s[kWarps - 1], kWarps, marked); }
-    __device__ __forceinline__ static Stretch joined(const Stretch (*q)[32], int n, bool marked) {
-        Stretch t = q[0][threadIdx.x & 31];
+    Stretch s[kWarps][32];
+    __device__ __forceinline__ Stretch& of(int place) { return s[place][threadIdx.x & 31]; }
+    // what the first `n` segments do together; `marked`: a start flag is among the tile's
+    __device__ __forceinline__ Stretch first(int n, bool marked) const {
+        Stretch t = Stretch::nothing();
         if (!marked) {
 #pragma unroll
-            for (int j = 1; j < n; ++j) {
-                const Stretch next = q[j][threadIdx.x & 31];
-                t = {mul2(t.A, next.A), next.of_uncut(t.b)};
-            }
+            for (int j = 0; j < kWarps; ++j)
+                if (j < n) {
+                    const Stretch next = s[j][threadIdx.x & 31];
+                    t = {mul2(t.A, next.A), next.of_uncut(t.b)};
+                }
         } else {
-            for (int j = 1; j < n; ++j) t = t.then(q[j][threadIdx.x & 31]);
+            for (int j = 0; j < n; ++j) t = t.then(s[j][threadIdx.x & 31]);
         }
         return t;
     }
@@ -308,13 +300,7 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
     for (int i = 0; i < kStages; ++i) ask(i);
     F2 carry = get_state(p.s0 != nullptr ? p.s0 + state : nullptr, at.channels);      // state entering the round (kTurn: the sequence)
     if (at.L == 0 && warp == 0 && rank == 0) put_state(s_out + state, carry, at.channels);
-    if constexpr (kTurn) {
-        ex.open();
-    } else {
-        chain[0].pad();
-        chain[1].pad();
-        ex.open(ranks);
-    }
+    ex.open();
     bool lost = false;
     const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)at.bi * p.T : nullptr;
     const uint32_t down = p.C * (uint32_t)sizeof(T), own_off = warp * kSeg * down + at.col * (uint32_t)sizeof(T);
@@ -358,8 +344,8 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
             if (plain) summarise(Plain()); else summarise(Marked());
             chain[parity].of(warp) = Stretch{A, b};
             const bool marked = __syncthreads_or(starts != 0);   // a start flag in the tile
-            if (warp == kWarps - 1) ex.send(round, rank, ranks, chain[parity].all(marked), lane);
-            const Stretch front = chain[parity].front(warp, marked);
+            if (warp == kWarps - 1) ex.send(round, rank, ranks, chain[parity].first(kWarps, marked), lane);
+            const Stretch front = chain[parity].first(warp, marked);
             ex.wait(round, lost, p.status);
 #pragma unroll
             for (int q = 0; q < kMaxCluster; ++q) {
@@ -432,13 +418,7 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
     for (int i = 0; i < kStages; ++i) ask(i);
     F2 next = entering(0), carry = both(0.f);                    // carry: c entering the round from behind
     const F2 gstate = get_state(gs != nullptr ? gs + state : nullptr, at.channels);
-    if constexpr (kTurn) {
-        ex.open();
-    } else {
-        back[0].pad();
-        back[1].pad();
-        ex.open(ranks);
-    }
+    ex.open();
     bool lost = false;
     const uint8_t* const ns = p.starts != nullptr ? p.starts + (size_t)at.bi * p.T : nullptr;
     const uint32_t down = p.C * (uint32_t)sizeof(T), own_off = warp * kSeg * down + at.col * (uint32_t)sizeof(T);
@@ -494,8 +474,8 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
             if (plain) summarise(Plain()); else summarise(Marked());
             back[parity].of(kWarps - 1 - warp) = Stretch{A, c};
             const bool marked = __syncthreads_or(starts != 0);   // a start flag in the tile
-            if (warp == 0) ex.send(done, rank, ranks, back[parity].all(marked), lane);
-            const Stretch rear = back[parity].front(kWarps - 1 - warp, marked);
+            if (warp == 0) ex.send(done, rank, ranks, back[parity].first(kWarps, marked), lane);
+            const Stretch rear = back[parity].first(kWarps - 1 - warp, marked);
             ex.wait(done, lost, p.status);
 #pragma unroll
             for (int q = kMaxCluster - 1; q >= 0; --q) {
@@ -600,8 +580,8 @@ struct Residency {
         return cfg;
     }
 };
-// CTAs of a cluster: those with which the last sequence is done soonest, by the rounds that it takes and the waves of clusters in front of it; the
-// smaller of equals.  One CTA alone passes the state from warp to warp and takes kAlone of a cluster's time for a round.  Forward / backward in us with
+// CTAs of a cluster: those with which the last sequence is done soonest, by the rounds that it takes (and one to begin with) and the waves of
+// clusters in front of it; the smaller of equals.  One CTA alone passes the state from warp to warp and takes kAlone of a cluster's time for a round.  Forward / backward in us with
 // one CTA a sequence and with clusters, bf16: B=4, T=1024, C=2048 20 / 29 and 25 / 31 (of two); B=16, T=512, C=768 16 / 22 and 27 / 33 (two); B=2,
 // T=8192, C=1024 98 / 156 and 35 / 51 (eight); B=1, T=2000, C=2560 30 and 21 (six); fp32, B=4, T=2048, C=2048 43 / 64 and 45 / 80 (two).  Narrow pieces take a warp longer to ask for:
 // fp32, B=3, T=1023, C=1001 31 / 57 and 23 / 35; bf16, B=4, T=2048, C=1001 92 / 139 and 37 / 57.  (`wide` goes by the row's length alone, so that
@@ -610,10 +590,10 @@ struct Residency {
 int ranks_of(const int* alone, const int* resident, long long units, int tiles, bool wide) {
     const double kAlone = wide ? 0.5 : 0.8;
     int best = 1;
-    double least = kAlone * ((units + alone[1] - 1) / alone[1]) * tiles;
+    double least = (double)((units + alone[1] - 1) / alone[1]) * (kAlone * tiles + 1);
     for (int n = 2; n <= kMaxCluster && n <= tiles; ++n) {
         if (resident[n] < 1) continue;
-        const double rounds = (double)((units + resident[n] - 1) / resident[n]) * ((tiles + n - 1) / n);
+        const double rounds = (double)((units + resident[n] - 1) / resident[n]) * ((tiles + n - 1) / n + 1);
         if (rounds < least) { least = rounds; best = n; }
     }
     return best;

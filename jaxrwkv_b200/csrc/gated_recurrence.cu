@@ -4,19 +4,27 @@
 //   h_t = (start_t ? 0 : a_t h_{t-1}) + u_t     out_t = h_t     s_out = h_{length-1}
 // Both gates lie in [0, 1], so a product of them over any stretch of tokens cannot overflow.
 //
-// The recurrence is associative: a stretch of tokens acts on the state entering it as h -> A h + b.  A CTA of eight warps owns
-// 64 channels of one sequence, a pair a lane, each warp consecutive segments of tokens, and the CTAs of a cluster own
-// consecutive tiles in turn:
-//   1. every warp turns its segment, which cp.async has brought into shared memory rounds ago, into gates and increments in
-//      registers, asks for the segment two rounds on, and reduces what it has to (A, b);
-//   2. the warps' (A, b) are combined in order through shared memory; where a cluster shares the sequence, the last warp sends
-//      the whole tile's to every CTA of it (st.async onto an mbarrier there), and everyone carries the state over all tiles of
-//      the round: one hop, whatever the size of the cluster;
-//   3. every warp walks its segment from the state that enters it and writes the outputs.
+// Memory bounds it: 3 elements a token and channel forward, 5 backward, and the kept states.  A CTA of eight warps owns 64 channels of one
+// sequence, two a lane, and its warps consecutive segments of 16 (fp32: 8) tokens, each of which
+//   1. turns its segment, which cp.async has brought into shared memory two rounds ago, into gates and increments in registers,
+//      and asks for the segment two rounds on;
+//   2. gets the state that enters the segment;
+//   3. walks the segment from that state and writes the outputs.
+// Where there are sequences enough for the device, a CTA has one to itself and step 2 is a box that the warp in front fills when it
+// has walked its segment (Mail): no warp waits for another but for that.  Forward / backward of B=8, T=4096, C=2048, bf16, sigmoid: 72 / 118 us,
+// 0.94 / 0.92 of the measured copy rate; 256 CTAs on 296 places.  A segment's way through the chain takes 333 cycles (265 backward), which
+// is what bounds a long sequence then: 11 ns a token.
+// Where there are fewer, a cluster of up to eight CTAs shares a sequence, tile by tile.  The recurrence is associative: a stretch of
+// tokens acts on the state entering it as h -> A h + b.  The warps reduce their segments to (A, b), the last one sends the whole tile's to
+// every CTA of the cluster (st.async onto an mbarrier there), and everyone carries the state over all tiles of the round: one hop,
+// whatever the size of the cluster.  One sequence of 32768 tokens, C=2048: 96 us in 32 clusters of eight, 0.65 of the copy rate; 48 % of issue slots,
+// the rest latency of a round's barrier and hop, which two CTAs an SM hide in part.
+// Segments of 16 tokens and a pair of channels a lane are what 128 registers hold; with 8 tokens the work around a segment makes the forward
+// 125 us instead of 82, with 16 warps a CTA 107 (both measured in the form with barriers).
 //
-// Backward: dh_t = gy_t + [t == length-1] gs + c_{t+1},  c_t = start_t ? 0 : a_t dh_t.  The states are recomputed from the
-// state entering each tile of 64 tokens, which the forward keeps (4 bytes per 64 tokens and channel); c runs over the segments
-// from the last to the first with the same products A.
+// Backward: dh_t = gy_t + [t == length-1] gs + c_{t+1},  c_t = start_t ? 0 : a_t dh_t.  The states are recomputed in segments of 8
+// tokens from the state entering each, which the forward keeps (4 bytes per 8 tokens and channel: a twelfth of a bf16 forward's traffic, a
+// twentieth of the backward's); c runs over the segments from the last to the first as the state does forward.
 //
 // A start flag cuts by a select, not by a factor of 0: what is no number in front of it ends there.
 #include <limits.h>
@@ -581,11 +589,11 @@ struct Residency {
     }
 };
 // CTAs of a cluster: those with which the last sequence is done soonest, by the rounds that it takes (and one to begin with) and the waves of
-// clusters in front of it; the smaller of equals.  One CTA alone passes the state from warp to warp and takes kAlone of a cluster's time for a round.  Forward / backward in us with
-// one CTA a sequence and with clusters, bf16: B=4, T=1024, C=2048 20 / 29 and 25 / 31 (of two); B=16, T=512, C=768 16 / 22 and 27 / 33 (two); B=2,
-// T=8192, C=1024 98 / 156 and 35 / 51 (eight); B=1, T=2000, C=2560 30 and 21 (six); fp32, B=4, T=2048, C=2048 43 / 64 and 45 / 80 (two).  Narrow pieces take a warp longer to ask for:
-// fp32, B=3, T=1023, C=1001 31 / 57 and 23 / 35; bf16, B=4, T=2048, C=1001 92 / 139 and 37 / 57.  (`wide` goes by the row's length alone, so that
-// results do not depend on where operands lie.)
+// clusters in front of it; the smaller of equals.  One CTA alone takes kAlone of a cluster's time for a round.  Forward / backward in us with one CTA a
+// sequence and with clusters, bf16: B=4, T=1024, C=2048 20 / 29 and 25 / 31 (of two); B=16, T=512, C=768 16 / 22 and 27 / 33 (two); B=2, T=8192,
+// C=1024 98 / 156 and 35 / 51 (eight); B=1, T=2000, C=2560 30 and 21 (six); fp32, B=4, T=2048, C=2048 43 / 64 and 45 / 80 (two).  Rows that
+// 16-byte pieces do not fit take a warp longer to ask for: fp32, B=3, T=1023, C=1001 31 / 57 and 23 / 35; bf16, B=4, T=2048, C=1001 92 / 139 and
+// 37 / 57.  (`wide` goes by the row's length alone, so that results do not depend on where operands lie.)
 // units: 64 channels of a sequence each; tiles: of one of them.
 int ranks_of(const int* alone, const int* resident, long long units, int tiles, bool wide) {
     const double kAlone = wide ? 0.5 : 0.8;

@@ -6,10 +6,14 @@
 //   dweight = sum over rows of dn xh   dbias = sum over rows of dn
 // The statistics are computed again in the backward (its x is read anyway), so nothing is kept.
 //
-// One pass over the rows, bound by memory.  A team of threads owns one group: a power of two of lanes of a warp with up to two
-// 16-byte pieces of the row each, or a whole CTA where the group is wider than that.  The row's values stay in registers from
-// the mean over the centred squares to the result.  A team keeps its group from row to row, so that weight and bias are read
-// once and their gradients are added up in registers; they leave as partial rows, which a second kernel adds in a fixed order.
+// One pass over the rows, bound by memory: 3 elements a channel forward, 5 backward (2 and 3 without a gate).  A team of threads owns one group: a
+// power of two of lanes of a warp with one or two 16-byte pieces of the row each (four pairs where 16 bytes do not fit), or a whole
+// CTA where the group is wider than that.  The row's values stay in registers from the mean over the centred squares to the
+// result.  A team keeps its group from row to row, so that weight and bias are read once and their gradients are added up in
+// registers; they leave as partial rows, which a second kernel adds in a fixed order.
+// 32768 rows of 32 groups of 64 channels, bf16, silu of a gate: forward 61 us, 1.02 of the measured copy rate; backward 110 us, 0.95, and
+// 4 us for the sums behind it.  Where groups are no power of two of pieces lanes stand idle (20 groups of 80: 0.63 of them work, forward 0.67 and
+// backward 0.57 of the copy rate, bound by issue slots).
 #include <initializer_list>
 #include <type_traits>
 

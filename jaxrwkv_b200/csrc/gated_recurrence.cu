@@ -48,7 +48,7 @@ constexpr int kWide = 64;                  // channels of a CTA
 constexpr int kKept = 8;                   // tokens per kept state, and of a backward segment
 constexpr int kMaxCluster = 8;
 constexpr int kStages = 2;
-constexpr int kWaitRanOut = 3;             // status word: a wait for the other CTAs of a cluster
+constexpr int kWaitRanOut = 3;             // status word: a wait for the warp in front, or for the other CTAs of a cluster
 
 // two channels, as they lie in shared memory
 __device__ __forceinline__ F2 pair_at(const float* p) { return *reinterpret_cast<const F2*>(p); }

@@ -102,50 +102,102 @@ struct alignas(16) Stretch {
 };
 
 // A CTA's tiles of one stream on their way to shared memory, each warp its segment: kSeg rows of 64 channels, zeros behind the sequence's
-// end and the last channel.  Pieces of kPiece bytes; 2: single 16-bit elements, which no asynchronous copy takes.  Addresses are a
-// base that is the same for the CTA and 32 bits of the lane's own, where a tile of whole rows is that near.
+// end and the last channel.  Addresses are a base that is the same for the CTA and 32 bits of the lane's own, where a tile of whole rows is
+// that near.  Rows travel as the 16-byte chunks that they lie in.
+__device__ __forceinline__ void copy_chunk(uint32_t to, const char* from, int valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid) : "memory");
+}
+// Rows that begin anywhere (kPiece 2 or 4: on what) are a chunk more, and what lies in front of them in it comes along unused (allocations begin
+// on 16 bytes, so it is there).  Forward / backward in us, in front of them with copies of 4 bytes and, for rows that begin on 2, of single elements:
+// bf16, B=1, T=8191, C=1001 64 / 98 and 47 / 75; B=16, T=1024, C=1001 54 / 86 and 37 / 53; B=4, T=2048, C=2046 48 / 72 and 40 / 61; fp32, B=8,
+// T=2048, C=1001 69 / 113 and 57 / 71.  (Words instead of elements for the outputs of such rows too: 51 / 88 -> 57 / 102, not taken.)
 template <typename T, int kPiece, int kSeg> struct Feed {
-    static constexpr int kPer = kPiece / (int)sizeof(T), kPerRow = kWide / kPer;
-    static constexpr int kRows = kPerRow <= 32 ? 32 / kPerRow : 1, kPasses = kPerRow <= 32 ? 1 : kPerRow / 32;
-    const char* base;                      // token 0 of the CTA's channels
+    static constexpr int kChunks = kWide * (int)sizeof(T) / 16, kRow = (kChunks + 1) * 16;      // of a row; bytes in shared memory
+    static constexpr int kRows = 32 / kChunks;                          // at a time
+    const char* base;                      // the chunk of the CTA's first channel in token 0
     long long stride;                      // bytes from token to token
-    uint32_t off;                          // the lane's first piece in a tile
+    uint32_t off;                          // the lane's first row in a tile
+    int shift, step;                       // of a row in its first chunk: of token 0, and from token to token
+    int bytes;                             // of the channels that there are
+    bool near;
+    __device__ __forceinline__ static int row() { return (int)(threadIdx.x & 31) / kChunks; }
+    __device__ __forceinline__ static int chunk() { return (int)(threadIdx.x & 31) % kChunks; }
+    __device__ __forceinline__ Feed(const void* p, long long batch, long long token, int bi, int c0, int C)
+        : base((const char*)p + (bi * batch + c0) * (long long)sizeof(T)), stride(token * (long long)sizeof(T)), bytes((C - c0) * (int)sizeof(T)) {
+        shift = (int)(uintptr_t)base & 15;
+        step = (int)stride & 15;
+        base -= shift;
+        off = (threadIdx.x / 32 * kSeg + row()) * (uint32_t)stride + shift;
+        near = stride * (kSeg * kWarps) < (1LL << 31) && bytes >= kRow;
+    }
+    // of the warp's i-th row (its segment begins at a multiple of eight tokens)
+    __device__ __forceinline__ int shift_of(int i) const { return (shift + i * step) & 15; }
+    // chunk k of the warp's i-th row, where not all of it may be there
+    __device__ __forceinline__ void edge(uint32_t to, int t0, int i, int k, int Tlen) const {
+        const int left = t0 + i < Tlen ? bytes + shift_of(i) - 16 * k : 0, valid = left < 0 ? 0 : left < 16 ? left : 16;
+        copy_chunk(to + i * kRow + 16 * k, base + (valid ? (((t0 + i) * stride + shift) & ~15LL) + 16 * k : 0), valid);
+    }
+    // the tile that begins at t0; `to`: the warp's rows in shared memory
+    __device__ __forceinline__ void fetch(uint32_t to, int t0, int Tlen) const {
+        const int seg = (int)(threadIdx.x / 32) * kSeg, lane = threadIdx.x & 31;
+        if (near && t0 + kSeg * kWarps <= Tlen) {
+            const char* const tile = base + t0 * stride;
+            const uint32_t down = (uint32_t)(kRows * stride), into = to + row() * kRow + 16 * chunk();
+            uint32_t at = off;
+#pragma unroll
+            for (int i = 0; i < kSeg; i += kRows, at += down) copy_chunk(into + i * kRow, tile + ((at & ~15u) + 16 * chunk()), 16);
+            if (lane < kSeg) copy_chunk(to + lane * kRow + 16 * kChunks, tile + ((((seg + lane) * (uint32_t)stride + shift) & ~15u) + 16 * kChunks), 16);
+        } else {
+            for (int i = 0; i < kSeg; i += kRows) edge(to, t0 + seg, i + row(), chunk(), Tlen);
+            if (lane < kSeg) edge(to, t0 + seg, lane, kChunks, Tlen);
+        }
+    }
+    // the lane's two channels of the warp's i-th row; `rows`: where they would be in the first one if it began on 16 bytes
+    __device__ __forceinline__ F2 at(const unsigned char* rows, int i) const {
+        const unsigned char* const q = rows + i * kRow + shift_of(i);
+        if constexpr (sizeof(T) == 4) {
+            return make_f2(((const float*)q)[0], ((const float*)q)[1]);
+        } else if constexpr (kPiece == 4) {
+            return pair_at((const __nv_bfloat16*)q);
+        } else {                           // a word, or the halves of two
+            const uint32_t half = (uint32_t)(uintptr_t)q & 2;
+            const uint32_t* const word = (const uint32_t*)(q - half);
+            return unpack_pair(__funnelshift_r(word[0], word[1], half * 8));
+        }
+    }
+};
+// Rows that begin on 16 bytes.
+template <typename T, int kSeg> struct Feed<T, 16, kSeg> {
+    static constexpr int kPer = 16 / (int)sizeof(T), kChunks = kWide / kPer, kRow = kChunks * 16, kRows = 32 / kChunks;
+    const char* base;                      // token 0 of the CTA's channels
+    long long stride;
+    uint32_t off;                          // the lane's first chunk in a tile
     int left;                              // channels that there are
     bool near;
-    __device__ __forceinline__ static int row() { return kPasses == 1 ? (int)(threadIdx.x & 31) / kPerRow : 0; }
-    __device__ __forceinline__ static int channel() { return (int)(kPasses == 1 ? (threadIdx.x & 31) % kPerRow : threadIdx.x & 31) * kPer; }
+    __device__ __forceinline__ static int row() { return (int)(threadIdx.x & 31) / kChunks; }
+    __device__ __forceinline__ static int channel() { return (int)(threadIdx.x & 31) % kChunks * kPer; }
     __device__ __forceinline__ Feed(const void* p, long long batch, long long token, int bi, int c0, int C)
         : base((const char*)p + (bi * batch + c0) * (long long)sizeof(T)), stride(token * (long long)sizeof(T)), left(C - c0) {
         near = stride * (kSeg * kWarps) < (1LL << 31) && left >= kWide;
         off = (uint32_t)((threadIdx.x / 32 * kSeg + row()) * (uint32_t)stride + channel() * sizeof(T));
     }
-    __device__ __forceinline__ static void piece(uint32_t to, const char* from, bool valid) {
-        if constexpr (kPiece == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
-        else if constexpr (kPiece == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(valid ? 4 : 0) : "memory");
-        else asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(valid ? *(const unsigned short*)from : (unsigned short)0) : "memory");
-    }
-    // the tile that begins at t0; `to`: the warp's rows in shared memory
     __device__ __forceinline__ void fetch(uint32_t to, int t0, int Tlen) const {
-        to += (row() * kWide + channel()) * sizeof(T);
+        to += row() * kRow + channel() * (int)sizeof(T);
         if (near && t0 + kSeg * kWarps <= Tlen) {
             const char* const tile = base + t0 * stride;
             const uint32_t down = (uint32_t)(kRows * stride);
             uint32_t at = off;
 #pragma unroll
-            for (int i = 0; i < kSeg; i += kRows, at += down)
-#pragma unroll
-                for (int pass = 0; pass < kPasses; ++pass) piece(to + (i * kWide + pass * 32 * kPer) * sizeof(T), tile + at + pass * 32 * kPiece, true);
+            for (int i = 0; i < kSeg; i += kRows, at += down) copy_chunk(to + i * kRow, tile + at, 16);
         } else {
             const int first = t0 + (int)(threadIdx.x / 32) * kSeg + row();
-            for (int i = 0; i < kSeg; i += kRows)
-#pragma unroll
-                for (int pass = 0; pass < kPasses; ++pass) {
-                    const int c = channel() + pass * 32 * kPer;
-                    const bool valid = first + i < Tlen && c < left;
-                    piece(to + (i * kWide + pass * 32 * kPer) * sizeof(T), base + (valid ? (first + i) * stride + c * (long long)sizeof(T) : 0), valid);
-                }
+            for (int i = 0; i < kSeg; i += kRows) {
+                const bool valid = first + i < Tlen && channel() < left;
+                copy_chunk(to + i * kRow, base + (valid ? (first + i) * stride + channel() * (long long)sizeof(T) : 0), valid ? 16 : 0);
+            }
         }
     }
+    __device__ __forceinline__ F2 at(const unsigned char* rows, int i) const { return pair_at((const T*)rows + i * kWide); }
 };
 __device__ __forceinline__ void fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void wait_fetched() {
@@ -286,7 +338,7 @@ constexpr int kBwdSeg = kKept;
 template <typename T, int kGate, int kPiece, bool kTurn>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, float* __restrict__ kept) {
-    constexpr int kSeg = kFwdSeg<T>, kTile = kSeg * kWarps, kRow = kWide * (int)sizeof(T), kRoom = 2 * kSeg * kRow;
+    constexpr int kSeg = kFwdSeg<T>, kTile = kSeg * kWarps, kRow = Feed<T, kPiece, kSeg>::kRow, kRoom = 2 * kSeg * kRow;
     extern __shared__ __align__(128) unsigned char dynamic[];
     __shared__ std::conditional_t<kTurn, Mail, Exchange> ex;
     __shared__ std::conditional_t<kTurn, char, Chain> chain[2];
@@ -319,12 +371,12 @@ gated_fwd_kernel(const Problem p, T* __restrict__ y, float* __restrict__ s_out, 
         // 1. gates and increments
         F2 a[kSeg], u[kSeg];
         wait_fetched<kStages - 1>();
-        const T* const from = (const T*)(room + round % kStages * kRoom) + at.col;
+        const unsigned char* const from = room + round % kStages * kRoom + at.col * (int)sizeof(T);
 #pragma unroll
         for (int i = 0; i < kSeg; ++i) {
-            const F2 x = pair_at(from + i * kWide);
+            const F2 x = fx.at(from, i);
             F2 w;
-            gate_of<T, kGate>(pair_at(from + (kSeg + i) * kWide), a[i], w);
+            gate_of<T, kGate>(ff.at(from + kSeg * kRow, i), a[i], w);
             u[i] = kGate == kSigmoidGate ? mul2(w, x) : x;
         }
         __syncwarp();                      // the segment has been read
@@ -393,7 +445,7 @@ template <typename T, int kGate, int kPiece, bool kTurn>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restrict__ gs, const float* __restrict__ kept,
                  T* __restrict__ dx, T* __restrict__ df, float* __restrict__ ds0) {
-    constexpr int kSeg = kBwdSeg, kTile = kSeg * kWarps, kRow = kWide * (int)sizeof(T), kRoom = 3 * kSeg * kRow;
+    constexpr int kSeg = kBwdSeg, kTile = kSeg * kWarps, kRow = Feed<T, kPiece, kSeg>::kRow, kRoom = 3 * kSeg * kRow;
     extern __shared__ __align__(128) unsigned char dynamic[];
     __shared__ std::conditional_t<kTurn, Mail, Exchange> ex;
     __shared__ std::conditional_t<kTurn, char, Chain> back[2];
@@ -440,12 +492,12 @@ gated_bwd_kernel(const Problem p, const T* __restrict__ gy, const float* __restr
         // 1. gates, states, and in the place of x what df is dx times of
         F2 a[kSeg], w[kSeg], x[kSeg], g[kSeg];
         wait_fetched<kStages - 1>();
-        const T* const from = (const T*)(room + done % kStages * kRoom) + at.col;
+        const unsigned char* const from = room + done % kStages * kRoom + at.col * (int)sizeof(T);
 #pragma unroll
         for (int i = 0; i < kSeg; ++i) {
-            x[i] = pair_at(from + i * kWide);
-            gate_of<T, kGate>(pair_at(from + (kSeg + i) * kWide), a[i], w[i]);
-            g[i] = pair_at(from + (2 * kSeg + i) * kWide);
+            x[i] = fx.at(from, i);
+            gate_of<T, kGate>(ff.at(from + kSeg * kRow, i), a[i], w[i]);
+            g[i] = fg.at(from + 2 * kSeg * kRow, i);
         }
         __syncwarp();                      // the segment has been read
         ask(done + kStages);
@@ -589,14 +641,13 @@ struct Residency {
     }
 };
 // CTAs of a cluster: those with which the last sequence is done soonest, by the rounds that it takes (and one to begin with) and the waves of
-// clusters in front of it; the smaller of equals.  One CTA alone takes kAlone of a cluster's time for a round.  Forward / backward in us with one CTA a
+// clusters in front of it; the smaller of equals.  One CTA alone takes half of a cluster's time for a round.  Forward / backward in us with one CTA a
 // sequence and with clusters, bf16: B=4, T=1024, C=2048 20 / 29 and 25 / 31 (of two); B=16, T=512, C=768 16 / 22 and 27 / 33 (two); B=2, T=8192,
-// C=1024 98 / 156 and 35 / 51 (eight); B=1, T=2000, C=2560 30 and 21 (six); fp32, B=4, T=2048, C=2048 43 / 64 and 45 / 80 (two).  Rows that
-// 16-byte pieces do not fit take a warp longer to ask for: fp32, B=3, T=1023, C=1001 31 / 57 and 23 / 35; bf16, B=4, T=2048, C=1001 92 / 139 and
-// 37 / 57.  (`wide` goes by the row's length alone, so that results do not depend on where operands lie.)
+// C=1024 98 / 156 and 35 / 51 (eight); B=1, T=2000, C=2560 30 and 21 (six); B=8, T=1024, C=1001 25 / 37 and 30 / 41 (two); fp32, B=4, T=2048, C=2048
+// 43 / 64 and 45 / 80 (two); B=8, T=2048, C=1001 49 / 73 and 55 / 107 (two); the rule's miss: B=3, T=1023, C=1001 backward 37 and 33 (two).
 // units: 64 channels of a sequence each; tiles: of one of them.
-int ranks_of(const int* alone, const int* resident, long long units, int tiles, bool wide) {
-    const double kAlone = wide ? 0.5 : 0.8;
+int ranks_of(const int* alone, const int* resident, long long units, int tiles) {
+    constexpr double kAlone = 0.5;
     int best = 1;
     double least = (double)((units + alone[1] - 1) / alone[1]) * (kAlone * tiles + 1);
     for (int n = 2; n <= kMaxCluster && n <= tiles; ++n) {
@@ -606,15 +657,32 @@ int ranks_of(const int* alone, const int* resident, long long units, int tiles, 
     }
     return best;
 }
-template <typename Kernel, typename... Args>
-int launch(Residency (&residency)[2], int row_bytes, Kernel turn, Kernel cluster, cudaStream_t st, const Problem& p, int tile, size_t smem, Args... args) {
-    const int *const alone = residency[0].of(turn, smem, 1), *const resident = residency[1].of(cluster, smem, kMaxCluster);
-    if (alone == nullptr || resident == nullptr || alone[1] < 1) return B200WKV_ELAUNCH;
-    const int slabs = (p.C + kWide - 1) / kWide, ranks = ranks_of(alone, resident, (long long)p.B * slabs, (p.T + tile - 1) / tile, row_bytes % 16 == 0);
+// A direction's two kernels, and how many of them the device takes.
+template <bool kForward, typename T, int kGate, int kPiece> struct Forms {
+    static constexpr int kSeg = kForward ? kFwdSeg<T> : kBwdSeg, kTile = kSeg * kWarps;
+    static constexpr size_t kSmem = (size_t)kStages * (kForward ? 2 : 3) * kTile * Feed<T, kPiece, kSeg>::kRow;
+    template <bool kTurn> static constexpr auto kernel() {
+        if constexpr (kForward) return &gated_fwd_kernel<T, kGate, kPiece, kTurn>;
+        else return &gated_bwd_kernel<T, kGate, kPiece, kTurn>;
+    }
+    static bool resident(const int*& alone, const int*& clusters) {
+        static Residency residency[2];
+        alone = residency[0].of(kernel<true>(), kSmem, 1);
+        clusters = residency[1].of(kernel<false>(), kSmem, kMaxCluster);
+        return alone != nullptr && clusters != nullptr && alone[1] >= 1;
+    }
+};
+template <bool kForward, typename T, int kGate, int kPiece, typename... Args> int launch(cudaStream_t st, const Problem& p, Args... args) {
+    typedef Forms<kForward, T, kGate, kPiece> F;
+    const int *alone, *clusters;
+    if (!F::resident(alone, clusters)) return B200WKV_ELAUNCH;
+    // (the choice goes by the length of the rows, so that results do not depend on where operands lie)
+    if (kPiece < 16 && p.C * sizeof(T) % 16 == 0 && !Forms<kForward, T, kGate, 16>::resident(alone, clusters)) return B200WKV_ELAUNCH;
+    const int slabs = (p.C + kWide - 1) / kWide, ranks = ranks_of(alone, clusters, (long long)p.B * slabs, (p.T + F::kTile - 1) / F::kTile);
     const unsigned y = p.B < 65535 ? p.B : 65535;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = Residency::config(attr, ranks, dim3((unsigned)slabs * ranks, y, (p.B + y - 1) / y), smem, st);
-    return cudaLaunchKernelEx(&cfg, ranks > 1 ? cluster : turn, p, args...) == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
+    const cudaLaunchConfig_t cfg = Residency::config(attr, ranks, dim3((unsigned)slabs * ranks, y, (p.B + y - 1) / y), F::kSmem, st);
+    return cudaLaunchKernelEx(&cfg, ranks > 1 ? F::template kernel<false>() : F::template kernel<true>(), p, args...) == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
 }
 // The widest pieces that every row of these begins on.
 int piece_of(int C, int element, std::initializer_list<const void*> streams, std::initializer_list<long long> strides) {
@@ -625,15 +693,11 @@ int piece_of(int C, int element, std::initializer_list<const void*> streams, std
 }
 
 template <typename T, int kGate, int kPiece> int fwd(cudaStream_t st, const Problem& p, void* y, float* s_out, float* kept) {
-    static Residency residency[2];
-    constexpr int kTile = kFwdSeg<T> * kWarps;
-    return launch(residency, p.C * (int)sizeof(T), gated_fwd_kernel<T, kGate, kPiece, true>, gated_fwd_kernel<T, kGate, kPiece, false>, st, p, kTile, (size_t)kStages * 2 * kTile * kWide * sizeof(T), (T*)y, s_out, kept);
+    return launch<true, T, kGate, kPiece>(st, p, (T*)y, s_out, kept);
 }
 template <typename T, int kGate, int kPiece>
 int bwd(cudaStream_t st, const Problem& p, const void* gy, const float* gs, const float* kept, void* dx, void* df, float* ds0) {
-    static Residency residency[2];
-    return launch(residency, p.C * (int)sizeof(T), gated_bwd_kernel<T, kGate, kPiece, true>, gated_bwd_kernel<T, kGate, kPiece, false>, st, p, kBwdSeg * kWarps, (size_t)kStages * 3 * kBwdSeg * kWarps * kWide * sizeof(T), (const T*)gy, gs, kept,
-                  (T*)dx, (T*)df, ds0);
+    return launch<false, T, kGate, kPiece>(st, p, (const T*)gy, gs, kept, (T*)dx, (T*)df, ds0);
 }
 // calls `go` with the element type, the gate and the piece as template arguments
 #define B200WKV_GATED_PIECE(go, T, piece, ...) \

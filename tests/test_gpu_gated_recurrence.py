@@ -337,3 +337,25 @@ def test_another_stream_and_captured_calls():
         for (x, f, s, length, ns, gy, gs), got in zip(fresh, outs):
             for a, b in zip(got, train(x, f, s, length, ns, "sigmoid", gs, gy)):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,C", [(19, 5), (70, 64), (150, 65), (150, 72), (300, 67), (600, 130)])
+def test_rows_that_begin_anywhere(T, C, dtype):
+    """Rows at every distance from 16 bytes, by where the tensor begins and by its token stride, amid values that are no numbers."""
+    B, gate = 2, "sigmoid"
+    x, f, s, length, ns, gy, gs = cuda(*inputs(B, T, C, gate, dtype, seed=T + C, starts=0.03))
+    want = train(x, f, s, length, ns, gate, gs, gy)
+    check_gated(want, x, f, s, length, ns, gate, gs, gy)
+
+    def placed(t, begin, apart):
+        room = torch.full((begin + B * T * apart,), float("nan"), dtype=dtype, device="cuda")
+        there = room[begin:].view(B, T, apart)[..., :C]
+        return there.copy_(t)
+
+    for begin in range(9):
+        px, pf = placed(x, begin, C + begin % 3), placed(f, 8 - begin, C + 7)
+        for a, b in zip(train(px, pf, s, length, ns, gate, gs, gy), want):
+            assert torch.equal(a, b)
+        s_out, out = gated_recurrence(px, pf, s, length, ns, gate=gate)
+        check_gated((s_out, out), x, f, s, length, ns, gate)

@@ -7,7 +7,7 @@
 // The statistics are computed again in the backward (its x is read anyway), so nothing is kept.
 //
 // One pass over the rows, bound by memory: 3 elements a channel forward, 5 backward (2 and 3 without a gate).  A team of threads owns one group: a
-// power of two of lanes of a warp with one or two 16-byte pieces of the row each (four pairs where 16 bytes do not fit), or a whole
+// power of two of lanes of a warp with one or two 16-byte pieces of the row each (up to eight pairs where 16 bytes do not fit), or a whole
 // CTA where the group is wider than that.  The row's values stay in registers from the mean over the centred squares to the
 // result.  A team keeps its group from row to row, so that weight and bias are read once and their gradients are added up in
 // registers; they leave as partial rows, which a second kernel adds in a fixed order.
@@ -271,12 +271,13 @@ template <typename Go> __device__ __forceinline__ void by_activation(int act, Go
     else go(std::integral_constant<int, B200WKV_ACT_NONE>());
 }
 
-// CTAs of 256 threads an SM for the registers of a kernel: weight, bias, a row's values and the next row's as they lie in memory
-constexpr int fwd_ctas(int elements, int bytes, bool gate) { return elements <= 4 || (elements <= 8 && bytes <= 16) ? 4 : elements <= 8 || !gate ? 3 : 2; }
-__host__ __device__ constexpr int bwd_ctas(int elements, bool gate) { return elements <= 4 ? 3 : elements <= 8 || !gate ? 2 : 1; }
+// CTAs of 256 threads an SM for the registers of a kernel: weight, bias, a row's values and the next row's as they lie in memory (`bytes`; a
+// register for each where they are loaded one by one)
+constexpr int fwd_ctas(int elements, int bytes, bool gate) { return elements <= 4 || (elements <= 8 && bytes <= 16) ? 4 : elements <= 8 || (!gate && bytes <= 32) ? 3 : 2; }
+__host__ __device__ constexpr int bwd_ctas(int elements, int bytes, bool gate) { return elements <= 4 ? 3 : elements <= 8 || (!gate && bytes <= 32) ? 2 : 1; }
 
 template <typename T, int VEC, int K, bool kWhole, bool kBlock, int kTeam, bool kGate>
-__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock && VEC * K <= 8 ? 2 : kBlock ? 1 : fwd_ctas(VEC * K, kWhole ? VEC * K * (int)sizeof(T) : 32, kGate))
+__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock && VEC * K <= 8 ? 2 : kBlock ? 1 : fwd_ctas(VEC * K, VEC * K * (kWhole ? (int)sizeof(T) : 4), kGate))
 group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
     typedef Lane<T, VEC, K, kWhole> L;
     __shared__ float room[kBlock ? 4 * kMaxThreads / 32 : 1];
@@ -325,7 +326,7 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
 }
 
 template <typename T, int VEC, int K, bool kWhole, bool kBlock, int kTeam, bool kGate>
-__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : bwd_ctas(VEC * K, kGate))
+__global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock ? 1 : bwd_ctas(VEC * K, VEC * K * (kWhole ? (int)sizeof(T) : 4), kGate))
 group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ partial) {
     typedef Lane<T, VEC, K, kWhole> L;
     constexpr int kPairs = L::kPairs;
@@ -472,7 +473,7 @@ Plan plan_of(Problem& p, int element, int aligned, bool forward) {
     q.whole = q.vec == wide || (aligned >= 2 * element && p.D % 2 == 0);
     const int pieces = (p.D + q.vec - 1) / q.vec;
     if (q.vec == wide) q.k = pieces <= 32 ? 1 : 2;
-    else q.k = 4;
+    else q.k = pieces <= 128 ? 4 : 8;      // bf16, 32768 rows of 4 groups of 333: forward / backward 223 / 282 us with CTAs of 64 and four pairs, 107 / 240 so
     if (pieces <= 32 * q.k) {
         q.block = 256;
         p.team = 1;
@@ -487,8 +488,10 @@ Plan plan_of(Problem& p, int element, int aligned, bool forward) {
     p.reduce = p.G * 4 <= teams;
     p.per_cta = p.reduce ? teams / p.G * p.G : teams;
     const long long all = p.rows * p.G;                  // rows of groups
-    // as many threads as the device has room for: a backward keeps its parameters' sums, so its CTAs are no more than are resident
-    const int threads = forward ? 2048 : q.vec * q.k <= 4 ? 768 : 512, ctas = threads > q.block ? threads / q.block : 1;
+    // as many threads as the device has room for: a backward keeps its parameters' sums, so its CTAs are no more than are resident (fp32, 16384
+    // rows of 2 groups of 1000, with one too many: 219 us, else 170)
+    const int elements = q.vec * q.k;
+    const int threads = forward ? 2048 : p.team > 32 ? 512 : 256 * bwd_ctas(elements, elements * (q.whole ? element : 4), p.gate != nullptr), ctas = threads > q.block ? threads / q.block : 1;
     const long long most_ctas = (long long)sm_count_of_current_device() * (ctas < 32 ? ctas : 32);
     long long grid = (all + p.per_cta - 1) / p.per_cta;
     if (!forward) {                        // four rows a team before there is a second CTA on an SM: each more is a partial row to add
@@ -552,10 +555,10 @@ template <typename T, typename Go> int dispatch(const Plan& q, const Problem& p,
         return gated(Wide(), Two(), Yes(), Yes(), Any());
     }
     if (q.whole) {
-        if (!block) return gated(Two(), Four(), Yes(), No(), Any());
+        if (!block) return q.k == 4 ? gated(Two(), Four(), Yes(), No(), Any()) : gated(Two(), Eight(), Yes(), No(), Warp());
         return q.k == 4 ? gated(Two(), Four(), Yes(), Yes(), Any()) : gated(Two(), Eight(), Yes(), Yes(), Any());
     }
-    if (!block) return gated(Two(), Four(), No(), No(), Any());
+    if (!block) return q.k == 4 ? gated(Two(), Four(), No(), No(), Any()) : gated(Two(), Eight(), No(), No(), Warp());
     return q.k == 4 ? gated(Two(), Four(), No(), Yes(), Any()) : gated(Two(), Eight(), No(), Yes(), Any());
 }
 template <typename T> int fwd(cudaStream_t st, Problem p, void* y) {

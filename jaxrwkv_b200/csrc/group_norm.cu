@@ -6,14 +6,15 @@
 //   dweight = sum over rows of dn xh   dbias = sum over rows of dn
 // The statistics are computed again in the backward (its x is read anyway), so nothing is kept.
 //
-// One pass over the rows, bound by memory: 3 elements a channel forward, 5 backward (2 and 3 without a gate).  A team of threads owns one group: a
-// power of two of lanes of a warp with one or two 16-byte pieces of the row each (up to eight pairs where 16 bytes do not fit), or a whole
+// One pass over the rows, bound by memory: 3 elements a channel forward, 5 backward (2 and 3 without a gate).  A team of threads owns one group: lanes
+// of a warp with one or two 16-byte pieces of the row each (up to eight pairs where 16 bytes do not fit), or a whole
 // CTA where the group is wider than that.  The row's values stay in registers from the mean over the centred squares to the
 // result.  A team keeps its group from row to row, so that weight and bias are read once and their gradients are added up in
 // registers; they leave as partial rows, which a second kernel adds in a fixed order.
 // 32768 rows of 32 groups of 64 channels, bf16, silu of a gate: forward 61 us, 1.02 of the measured copy rate; backward 110 us, 0.95, and
-// 4 us for the sums behind it.  Where groups are no power of two of pieces lanes stand idle (20 groups of 80: 0.63 of them work, forward 0.67 and
-// backward 0.57 of the copy rate, bound by issue slots).
+// 4 us for the sums behind it.  Groups that are no power of two of pieces leave lanes idle (24 groups of 72: 5 of 32) and take longer sums: 20
+// groups of 80 reach 0.73 and 0.71 of the copy rate, bound by issue slots.  Single elements, as of 32 groups of 61, reach 0.40 and 0.41, bound by
+// the number of loads.
 #include <initializer_list>
 #include <type_traits>
 
@@ -140,13 +141,41 @@ template <typename T, int kAct> __device__ __forceinline__ void activate(F2 z, F
     dp = kAct == B200WKV_ACT_SIGMOID ? mul2(s, r) : mul2(s, fma2(z, r, both(1.f)));
 }
 
+// Where a thread's team works: group g, rows first, first + parallel, ...; none of them where `at_work` is false.  A warp has as many teams as fit
+// it, and the lanes behind them are idle.
+struct Place {
+    int team, g, lane;
+    int slot;                              // teams' lanes in a row; -1: idle
+    long long first;
+    bool at_work;
+    __device__ __forceinline__ Place(const Problem& p, int team_) : team(team_) {
+        const int per_warp = 32 / team, in_warp = (int)(threadIdx.x & 31) / team;      // (0 and 0 for whole CTAs)
+        const int in_cta = team > 32 ? 0 : (int)(threadIdx.x / 32) * per_warp + in_warp, q = blockIdx.x * p.per_cta + in_cta;
+        lane = team > 32 ? (int)threadIdx.x : (int)(threadIdx.x & 31) - in_warp * team;
+        slot = team > 32 || in_warp < per_warp ? in_cta * team + lane : -1;
+        g = q % p.G;
+        first = q / p.G;
+        at_work = slot >= 0 && in_cta < p.per_cta && first < p.parallel;
+    }
+};
+
 // sum over the team, the same in every thread of it.  Whole CTAs: a row's sums have places of their own in `room`, so that one barrier
 // each is enough (a place is written again behind the barrier of the next sum, which everyone reaches after reading it).
-// kTeam: the team's lanes where they are known to the compiler, else 0 (five branches a sum).
-template <bool kBlock, int kTeam> __device__ __forceinline__ float team_sum(float a, int team, float* room) {
+// kTeam: the team's lanes where they are known to the compiler, 0 for any power of two (five branches a sum), kAnyTeam for others.
+constexpr int kAnyTeam = -1;
+template <bool kBlock, int kTeam> __device__ __forceinline__ float team_sum(float a, const Place& at, float* room) {
+    if (kTeam == kAnyTeam) {               // the first lane's is the team's
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            if (o >= at.team) break;
+            const float next = __shfl_down_sync(0xffffffffu, a, o);
+            if (at.lane + o < at.team) a += next;
+        }
+        return __shfl_sync(0xffffffffu, a, (int)(threadIdx.x & 31) - at.lane);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o /= 2)
-        if (kBlock || (kTeam ? kTeam : team) > o) a += __shfl_xor_sync(0xffffffffu, a, o);
+        if (kBlock || (kTeam > 0 ? kTeam : at.team) > o) a += __shfl_xor_sync(0xffffffffu, a, o);
     if (kBlock) {
         const int warps = blockDim.x / 32;
         if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = a;
@@ -156,20 +185,6 @@ template <bool kBlock, int kTeam> __device__ __forceinline__ float team_sum(floa
     }
     return a;
 }
-
-// Where a thread's team works: group g, rows first, first + parallel, ...; none of them where `at_work` is false
-struct Place {
-    int team, g, lane;
-    long long first;
-    bool at_work;
-    __device__ __forceinline__ Place(const Problem& p, int team_) : team(team_) {
-        const int in_cta = (int)threadIdx.x / team, q = blockIdx.x * p.per_cta + in_cta;
-        lane = (int)threadIdx.x % team;
-        g = q % p.G;
-        first = q / p.G;
-        at_work = in_cta < p.per_cta && first < p.parallel;
-    }
-};
 
 // The pieces of one thread: K, `step` channels apart.  kWhole false: the group's last element may be the first of a pair (`odd`).
 template <typename T, int VEC, int K, bool kWhole> struct Lane {
@@ -194,13 +209,13 @@ template <typename T, int VEC, int K, bool kWhole> struct Lane {
     }
     __device__ __forceinline__ void store(T* row, int k, const F2* v) const { P::store(row + k * step, v, second[k]); }
     // x less its mean over the team (0 where there is nothing), and 1 / sqrt(var + eps)
-    template <bool kBlock, int kTeam> __device__ __forceinline__ float centre(F2 (&x)[K][kPairs], const Problem& p, float inv_d, float* room) const {
+    template <bool kBlock, int kTeam> __device__ __forceinline__ float centre(F2 (&x)[K][kPairs], const Problem& p, const Place& at, float inv_d, float* room) const {
         F2 sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) sums = add2(sums, x[k][j]);
-        const F2 less = both(-team_sum<kBlock, kTeam>(sum_of(sums), p.team, room) * inv_d);
+        const F2 less = both(-team_sum<kBlock, kTeam>(sum_of(sums), at, room) * inv_d);
         sums = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -213,7 +228,7 @@ template <typename T, int VEC, int K, bool kWhole> struct Lane {
             }
             if (there[k]) sums = add2(sums, squares);
         }
-        return rsqrtf(team_sum<kBlock, kTeam>(sum_of(sums), p.team, room + kMaxThreads / 32) * inv_d + p.eps);
+        return rsqrtf(team_sum<kBlock, kTeam>(sum_of(sums), at, room + kMaxThreads / 32) * inv_d + p.eps);
     }
 };
 // A stream's pieces of the rows to come.  kAsync: pieces of 16 bytes travel to shared memory by cp.async, three rows in front of the one at
@@ -281,7 +296,7 @@ __global__ void __launch_bounds__(kBlock ? kMaxThreads : 256, kBlock && VEC * K 
 group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
     typedef Lane<T, VEC, K, kWhole> L;
     __shared__ float room[kBlock ? 4 * kMaxThreads / 32 : 1];
-    const Place at(p, kBlock ? (int)blockDim.x : kTeam ? kTeam : p.team);
+    const Place at(p, kBlock ? (int)blockDim.x : kTeam > 0 ? kTeam : p.team);
     const L my(p, at);
     const float inv_d = 1.f / (float)p.D;
     extern __shared__ __align__(16) unsigned char shared[];
@@ -306,7 +321,7 @@ group_norm_fwd_kernel(const Problem p, T* __restrict__ y) {
         if (kGate) rg.take(place, g, my);
         ask(place, row + (long long)R::kAhead * p.parallel);
         place = place + 1 == R::kAhead ? 0 : place + 1;
-        const F2 rstd = both(my.template centre<kBlock, kTeam>(x, p, inv_d, room));
+        const F2 rstd = both(my.template centre<kBlock, kTeam>(x, p, at, inv_d, room));
         by_activation(p.act, [&](auto act) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -331,7 +346,7 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     typedef Lane<T, VEC, K, kWhole> L;
     constexpr int kPairs = L::kPairs;
     __shared__ float room[kBlock ? 4 * kMaxThreads / 32 : 1];
-    const Place at(p, kBlock ? (int)blockDim.x : kTeam ? kTeam : p.team);
+    const Place at(p, kBlock ? (int)blockDim.x : kTeam > 0 ? kTeam : p.team);
     const L my(p, at);
     const float inv_d = 1.f / (float)p.D;
     F2 dw[K][kPairs], db[K][kPairs];
@@ -363,7 +378,7 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
         if (kGate) rg.take(place, g, my);
         ask(place, row + (long long)R::kAhead * p.parallel);
         place = place + 1 == R::kAhead ? 0 : place + 1;
-        const F2 rstd = both(my.template centre<kBlock, kTeam>(x, p, inv_d, room));
+        const F2 rstd = both(my.template centre<kBlock, kTeam>(x, p, at, inv_d, room));
         F2 s1 = both(0.f), s2 = both(0.f);                // of dxh and dxh xh
         by_activation(p.act, [&](auto act) {
 #pragma unroll
@@ -387,8 +402,8 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
                 }
             }
         });
-        const F2 m1 = both(-team_sum<kBlock, kTeam>(sum_of(s1), p.team, room + 2 * kMaxThreads / 32) * inv_d);
-        const F2 m2 = both(-team_sum<kBlock, kTeam>(sum_of(s2), p.team, room + 3 * kMaxThreads / 32) * inv_d);
+        const F2 m1 = both(-team_sum<kBlock, kTeam>(sum_of(s1), at, room + 2 * kMaxThreads / 32) * inv_d);
+        const F2 m2 = both(-team_sum<kBlock, kTeam>(sum_of(s2), at, room + 3 * kMaxThreads / 32) * inv_d);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (!my.there[k] || !on) continue;
@@ -408,8 +423,9 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
             __syncthreads();
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                both_sums[threadIdx.x * VEC + v] = of(dw[k], v);
-                both_sums[(256 + threadIdx.x) * VEC + v] = of(db[k], v);
+                if (at.slot < 0) continue;
+                both_sums[at.slot * VEC + v] = of(dw[k], v);
+                both_sums[(256 + at.slot) * VEC + v] = of(db[k], v);
             }
             __syncthreads();
             const int width = p.team * VEC, columns = 2 * p.G * width;         // of this k
@@ -476,19 +492,21 @@ Plan plan_of(Problem& p, int element, int aligned, bool forward) {
     else q.k = pieces <= 128 ? 4 : 8;      // bf16, 32768 rows of 4 groups of 333: forward / backward 223 / 282 us with CTAs of 64 and four pairs, 107 / 240 so
     if (pieces <= 32 * q.k) {
         q.block = 256;
+        const int lanes = (pieces + q.k - 1) / q.k;
         p.team = 1;
-        while (p.team * q.k < pieces) p.team *= 2;
+        while (p.team < lanes) p.team *= 2;
+        if (32 / lanes > 32 / p.team) p.team = lanes;    // bf16, 20 groups of 80, gated: 72 / 140 -> 67 / 116 us; 24 of 72: 86 / 163 -> 74 / 133; 32 of 48: 61 / 110 and 67 / 106
     } else {
         if (q.vec == wide) q.k = pieces <= kMaxThreads ? 1 : pieces <= 2 * kMaxThreads ? 2 : 4;
         else q.k = pieces <= 4 * kMaxThreads ? 4 : 8;
         q.block = ((pieces + q.k - 1) / q.k + 31) / 32 * 32;
         p.team = q.block;
     }
-    const int teams = q.block / p.team;
+    const int teams = p.team > 32 ? 1 : q.block / 32 * (32 / p.team);
     p.reduce = p.G * 4 <= teams;
     p.per_cta = p.reduce ? teams / p.G * p.G : teams;
     const long long all = p.rows * p.G;                  // rows of groups
-    // as many threads as the device has room for: a backward keeps its parameters' sums, so its CTAs are no more than are resident (fp32, 16384
+    // as many threads as the device has room for: a backward keeps its parameters' sums, so its CTAs are no more than are resident (fp32, 16777
     // rows of 2 groups of 1000, with one too many: 219 us, else 170)
     const int elements = q.vec * q.k;
     const int threads = forward ? 2048 : p.team > 32 ? 512 : 256 * bwd_ctas(elements, elements * (q.whole ? element : 4), p.gate != nullptr), ctas = threads > q.block ? threads / q.block : 1;
@@ -529,6 +547,7 @@ template <typename T, typename Go> int dispatch(const Plan& q, const Problem& p,
     typedef std::true_type Yes;
     typedef std::false_type No;
     typedef std::integral_constant<int, 0> Any;
+    typedef std::integral_constant<int, kAnyTeam> Other;
     typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, 2> Two;
     typedef std::integral_constant<int, 4> Four;
@@ -539,13 +558,14 @@ template <typename T, typename Go> int dispatch(const Plan& q, const Problem& p,
     const auto gated = [&](auto vec, auto k, auto whole, auto block, auto team) {
         return p.gate != nullptr ? go(vec, k, whole, block, team, Yes()) : go(vec, k, whole, block, team, No());
     };
-    const bool block = p.team > 32;
+    const bool block = p.team > 32, other = (p.team & (p.team - 1)) != 0;
     if (q.vec == kWide) {
         if (!block) {
             if (q.k == 2) return gated(Wide(), Two(), Yes(), No(), Warp());    // (more than 32 pieces)
             return p.team == 32   ? gated(Wide(), One(), Yes(), No(), Warp())
                    : p.team == 16 ? gated(Wide(), One(), Yes(), No(), Sixteen())
                    : p.team == 8  ? gated(Wide(), One(), Yes(), No(), Eight())
+                   : other        ? gated(Wide(), One(), Yes(), No(), Other())
                                   : gated(Wide(), One(), Yes(), No(), Any());
         }
         if (q.k == 1) return gated(Wide(), One(), Yes(), Yes(), Any());
@@ -555,10 +575,10 @@ template <typename T, typename Go> int dispatch(const Plan& q, const Problem& p,
         return gated(Wide(), Two(), Yes(), Yes(), Any());
     }
     if (q.whole) {
-        if (!block) return q.k == 4 ? gated(Two(), Four(), Yes(), No(), Any()) : gated(Two(), Eight(), Yes(), No(), Warp());
+        if (!block) return q.k == 8 ? gated(Two(), Eight(), Yes(), No(), Warp()) : other ? gated(Two(), Four(), Yes(), No(), Other()) : gated(Two(), Four(), Yes(), No(), Any());
         return q.k == 4 ? gated(Two(), Four(), Yes(), Yes(), Any()) : gated(Two(), Eight(), Yes(), Yes(), Any());
     }
-    if (!block) return q.k == 4 ? gated(Two(), Four(), No(), No(), Any()) : gated(Two(), Eight(), No(), No(), Warp());
+    if (!block) return q.k == 8 ? gated(Two(), Eight(), No(), No(), Warp()) : other ? gated(Two(), Four(), No(), No(), Other()) : gated(Two(), Four(), No(), No(), Any());
     return q.k == 4 ? gated(Two(), Four(), No(), Yes(), Any()) : gated(Two(), Eight(), No(), Yes(), Any());
 }
 template <typename T> int fwd(cudaStream_t st, Problem p, void* y) {

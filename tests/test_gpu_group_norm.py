@@ -216,3 +216,17 @@ def test_a_mixer_of_both(dtype):
         _, y1 = gated_recurrence_step(x1, f1, state, inplace=True)
         o1 = group_norm_act(y1, weight, bias, G, gate=g1, eps=64e-5)
     check_norm([o1], y1, weight, bias, G, g1, "silu", 64e-5)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,G,D", [(37, 7, 24), (301, 2, 24), (60, 9, 40), (9, 20, 80), (333, 1, 72), (700, 3, 48), (41, 3, 20), (50, 5, 44), (19, 13, 76),
+                                      (2000, 2, 20), (21, 4, 257), (30, 3, 333), (9, 4, 334), (5, 2, 511), (6, 2, 510), (8, 5, 260), (100, 1, 131)])
+def test_teams_of_any_size(rows, G, D, dtype, gated):
+    """Groups that take three, five, six, seven, nine, ten and more lanes, and single channels up to the widest that a warp has."""
+    x, w, b, gate, gy = make(rows, G * D, dtype, seed=rows + G + D)
+    gate = gate if gated else None
+    got = train(x, w, b, G, gate, "silu", 1e-3, gy)
+    check_norm(got, x, w, b, G, gate, "silu", 1e-3, gy)
+    with torch.no_grad():
+        assert torch.equal(group_norm_act(x, w, b, G, gate=gate, eps=1e-3), got[0])

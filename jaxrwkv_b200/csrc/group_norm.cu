@@ -27,6 +27,7 @@
 namespace b200wkv {
 namespace {
 
+constexpr int kChain = 16;                 // rows that a thread adds up in registers
 constexpr int kMaxPartials = 1024;         // partial rows of the parameters' gradients
 constexpr int kMaxThreads = 512;
 
@@ -72,6 +73,7 @@ struct Problem {
     int per_cta;                           // teams at work in a CTA: all of them, or a multiple of G
     int parallel;                          // rows at a time over the grid
     int param_vectors;                     // weight and bias begin on 16 bytes
+    int totals;                            // where the threads' sums beyond kChain rows begin in shared memory; -1: nobody takes so many
     int reduce;                            // teams of one group within a CTA are added up (per_cta is a multiple of G)
 };
 
@@ -280,6 +282,56 @@ template <int kAhead, bool kAsync> __device__ __forceinline__ void arrived() {
     if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
 }
 
+// A thread's sums of the parameters' gradients beyond kChain rows, in shared memory: 32768 rows are 111 a thread, and one chain of 32-bit additions
+// over them is three times as far off as the terms are.  kExact: with what each addition rounds away, which the next one makes up for (Kahan's
+// sum); else without, where the registers of a whole CTA have spilled and want the L1 cache (5120 channels: a pass 329 us, with 392).  dweight and
+// dbias of 32768 rows of 32 groups of 64, bf16 streams: 1.1e-7 and 1.0e-7 off (2-norm) instead of 2.2e-7, the terms alone are 0.8e-7 and 0.5e-7;
+// with 8 rows at a time 1.0e-7 and 0.9e-7, and 2 us more.  The pass through autograd 187 -> 185 us, without a gate 144 -> 153,
+// 8192 rows of 5120 channels 317 -> 329, 16384 rows of 2048 148 -> 154, fp32 rows of 2 groups of 1000 246 -> 241, others within 2.5 %.
+template <int kPairs, bool kExact, int kThreads> struct Totals {
+    struct alignas(kExact ? 16 : 8) Sum { F2 v[kExact ? 2 : 1]; };       // the sum, and what it is too large by
+    Sum* at;
+    bool on;
+    __device__ __forceinline__ Totals(unsigned char* shared, int from) : at((Sum*)(shared + from) + threadIdx.x), on(from >= 0) {}
+    __device__ __forceinline__ static int apart() { return kThreads > 0 ? kThreads : blockDim.x; }
+    __device__ __forceinline__ static F2 less(F2 a, F2 b) { return fma2(b, both(-1.f), a); }
+    // (an infinite sum stays one)
+    __device__ __forceinline__ static F2 of_finite(F2 s, F2 v) {
+        const float2 a = parts(s), b = parts(v);
+        return make_f2(isfinite(a.x) ? b.x : 0.f, isfinite(a.y) ? b.y : 0.f);
+    }
+    __device__ __forceinline__ static F2& of(F2* dw, F2* db, int i) { return i < kPairs ? dw[i] : db[i - kPairs]; }
+    // what the registers hold, which begin anew
+    __device__ __forceinline__ void add(F2* dw, F2* db, bool first) {
+#pragma unroll
+        for (int i = 0; i < 2 * kPairs; ++i) {
+            F2& v = of(dw, db, i);
+            Sum t = {};
+            if (!first) t = at[i * apart()];
+            if constexpr (kExact) {
+                const F2 y = less(v, t.v[1]), s = add2(t.v[0], y);
+                t = {{s, of_finite(s, less(less(s, t.v[0]), y))}};
+            } else {
+                t.v[0] = add2(t.v[0], v);
+            }
+            at[i * apart()] = t;
+            v = both(0.f);
+        }
+    }
+    // all of it, in the registers
+    __device__ __forceinline__ void take(F2* dw, F2* db) const {
+#pragma unroll
+        for (int i = 0; i < 2 * kPairs; ++i) {
+            F2& v = of(dw, db, i);
+            const Sum t = at[i * apart()];
+            if constexpr (kExact) v = less(v, t.v[1]);
+            v = add2(t.v[0], v);
+        }
+    }
+};
+
+template <int kPairs, bool kExact> constexpr size_t kTotalBytes = 2 * kPairs * (kExact ? 16 : 8);      // a thread's
+
 template <typename Go> __device__ __forceinline__ void by_activation(int act, Go go) {
     if (act == B200WKV_ACT_SILU) go(std::integral_constant<int, B200WKV_ACT_SILU>());
     else if (act == B200WKV_ACT_SIGMOID) go(std::integral_constant<int, B200WKV_ACT_SIGMOID>());
@@ -357,6 +409,9 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     extern __shared__ __align__(16) unsigned char shared[];
     constexpr bool kAsync = VEC == 8 && kAsyncRows<T, K, kWhole, kBlock, false>;
     typedef Rows<T, VEC, K, kWhole, kAsync> R;
+    const long long steps = (p.rows + p.parallel - 1) / p.parallel;
+    typedef Totals<K * kPairs, !(kBlock && K * kPairs > 4), kBlock ? 0 : 256> Sums;
+    Sums totals(shared, p.totals);
     R rx(p.x, p.x_stride, p, at, my, 0, shared), rd(gy, p.C, p, at, my, 1, shared), rg(p.gate, p.gate_stride, p, at, my, 2, shared);
     const auto ask = [&](int place, long long row) {
         rx.ask(place, row < p.rows, my);
@@ -366,54 +421,58 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
     };
     for (int i = 0; i < R::kAhead; ++i) ask(i, at.first + (long long)i * p.parallel);
     long long dense = at.first * p.C + my.c;
-    const long long steps = (p.rows + p.parallel - 1) / p.parallel;
     long long row = at.first;
     int place = 0;
-    for (long long i = 0; i < steps; ++i, row += p.parallel, dense += (long long)p.parallel * p.C) {
-        const bool on = row < p.rows;
-        F2 x[K][kPairs], g[K][kPairs], d[K][kPairs];
-        arrived<R::kAhead, kAsync>();
-        rx.take(place, x, my);
-        rd.take(place, d, my);
-        if (kGate) rg.take(place, g, my);
-        ask(place, row + (long long)R::kAhead * p.parallel);
-        place = place + 1 == R::kAhead ? 0 : place + 1;
-        const F2 rstd = both(my.template centre<kBlock, kTeam>(x, p, at, inv_d, room));
-        F2 s1 = both(0.f), s2 = both(0.f);                // of dxh and dxh xh
-        by_activation(p.act, [&](auto act) {
+    for (long long begin = 0; begin < steps; begin += kChain) {
+        if (totals.on && begin > 0) totals.add(&dw[0][0], &db[0][0], begin == kChain);
+        const int n = (int)(steps - begin < kChain ? steps - begin : kChain);
+        for (int i = 0; i < n; ++i, row += p.parallel, dense += (long long)p.parallel * p.C) {
+            const bool on = row < p.rows;
+            F2 x[K][kPairs], g[K][kPairs], d[K][kPairs];
+            arrived<R::kAhead, kAsync>();
+            rx.take(place, x, my);
+            rd.take(place, d, my);
+            if (kGate) rg.take(place, g, my);
+            ask(place, row + (long long)R::kAhead * p.parallel);
+            place = place + 1 == R::kAhead ? 0 : place + 1;
+            const F2 rstd = both(my.template centre<kBlock, kTeam>(x, p, at, inv_d, room));
+            F2 s1 = both(0.f), s2 = both(0.f);                // of dxh and dxh xh
+            by_activation(p.act, [&](auto act) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (!my.there[k] || !on) continue;
+#pragma unroll
+                    for (int j = 0; j < kPairs; ++j) {
+                        const F2 xh = mul2(x[k][j], rstd), n = fma2(xh, my.w[k][j], my.b[k][j]);
+                        F2 a, da;
+                        activate<T, act.value>(kGate ? g[k][j] : n, a, da);
+                        F2 dn = mul2(d[k][j], kGate ? a : da);
+                        if (kGate) g[k][j] = mul2(mul2(d[k][j], n), da);
+                        if (!kWhole && !my.second[k]) dn = first_alone(dn);
+                        dw[k][j] = fma2(dn, xh, dw[k][j]);
+                        db[k][j] = add2(db[k][j], dn);
+                        const F2 dxh = mul2(dn, my.w[k][j]);
+                        s1 = add2(s1, dxh);
+                        s2 = fma2(dxh, xh, s2);
+                        x[k][j] = xh;
+                        d[k][j] = dxh;
+                    }
+                }
+            });
+            const F2 m1 = both(-team_sum<kBlock, kTeam>(sum_of(s1), at, room + 2 * kMaxThreads / 32) * inv_d);
+            const F2 m2 = both(-team_sum<kBlock, kTeam>(sum_of(s2), at, room + 3 * kMaxThreads / 32) * inv_d);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (!my.there[k] || !on) continue;
+                if (kGate) my.store(dgate + dense, k, g[k]);
 #pragma unroll
-                for (int j = 0; j < kPairs; ++j) {
-                    const F2 xh = mul2(x[k][j], rstd), n = fma2(xh, my.w[k][j], my.b[k][j]);
-                    F2 a, da;
-                    activate<T, act.value>(kGate ? g[k][j] : n, a, da);
-                    F2 dn = mul2(d[k][j], kGate ? a : da);
-                    if (kGate) g[k][j] = mul2(mul2(d[k][j], n), da);
-                    if (!kWhole && !my.second[k]) dn = first_alone(dn);
-                    dw[k][j] = fma2(dn, xh, dw[k][j]);
-                    db[k][j] = add2(db[k][j], dn);
-                    const F2 dxh = mul2(dn, my.w[k][j]);
-                    s1 = add2(s1, dxh);
-                    s2 = fma2(dxh, xh, s2);
-                    x[k][j] = xh;
-                    d[k][j] = dxh;
-                }
+                for (int j = 0; j < kPairs; ++j) d[k][j] = mul2(fma2(x[k][j], m2, add2(d[k][j], m1)), rstd);
+                my.store(dx + dense, k, d[k]);
             }
-        });
-        const F2 m1 = both(-team_sum<kBlock, kTeam>(sum_of(s1), at, room + 2 * kMaxThreads / 32) * inv_d);
-        const F2 m2 = both(-team_sum<kBlock, kTeam>(sum_of(s2), at, room + 3 * kMaxThreads / 32) * inv_d);
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            if (!my.there[k] || !on) continue;
-            if (kGate) my.store(dgate + dense, k, g[k]);
-#pragma unroll
-            for (int j = 0; j < kPairs; ++j) d[k][j] = mul2(fma2(x[k][j], m2, add2(d[k][j], m1)), rstd);
-            my.store(dx + dense, k, d[k]);
         }
     }
     if (partial == nullptr) return;
+    if (totals.on) totals.take(&dw[0][0], &db[0][0]);
     // partial rows (parallel or one per CTA, 2, C): weight, bias
     const auto of = [](const F2* v, int i) { return i % 2 == 0 ? parts(v[i / 2]).x : parts(v[i / 2]).y; };
     if (!kBlock && p.reduce) {             // teams of one group within the CTA are added first, a column a thread
@@ -432,9 +491,9 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
             for (int t = threadIdx.x; t < columns; t += 256) {
                 const int which = t / (p.G * width), g = t % (p.G * width) / width, d = t % width, c = d + k * width;
                 if (c >= p.D) continue;
-                float sum = 0.f;
+                double sum = 0.;
                 for (int j = g; j < p.per_cta; j += p.G) sum += both_sums[which * 256 * VEC + j * width + d];
-                partial[((size_t)blockIdx.x * 2 + which) * p.C + g * p.D + c] = sum;
+                partial[((size_t)blockIdx.x * 2 + which) * p.C + g * p.D + c] = (float)sum;
             }
         }
         return;
@@ -451,12 +510,12 @@ group_norm_bwd_kernel(const Problem p, const T* __restrict__ gy, T* __restrict__
         }
 }
 
-// The partial rows' sums, in the parameters' type: a CTA owns 32 of the 2 C columns, its warps every sixteenth row, added in a fixed order.
+// The partial rows' sums, in 64 bits and rounded to the parameters' type: a CTA owns 32 of the 2 C columns, its warps every sixteenth row, added in a fixed order.
 __global__ void __launch_bounds__(512) group_norm_sums_kernel(const float* partial, int rows, int C, int f32, void* dweight, void* dbias) {
-    __shared__ float part[16][32];
+    __shared__ double part[16][32];
     wait_for_grid_in_front();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    float s[8] = {};
+    double s[8] = {};
     if (c < 2 * C)
         for (int r = warp; r < rows; r += 128)
 #pragma unroll
@@ -465,14 +524,14 @@ __global__ void __launch_bounds__(512) group_norm_sums_kernel(const float* parti
     part[warp][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (warp != 0 || c >= 2 * C) return;
-    float t = 0.f;
+    double t = 0.;
 #pragma unroll
     for (int w = 0; w < 16; ++w) t += part[w][lane];
     void* const to = c < C ? dweight : dbias;
     if (to == nullptr) return;
     const int at = c < C ? c : c - C;
-    if (f32) ((float*)to)[at] = t;
-    else ((__nv_bfloat16*)to)[at] = __float2bfloat16_rn(t);
+    if (f32) ((float*)to)[at] = (float)t;
+    else ((__nv_bfloat16*)to)[at] = __double2bfloat16(t);
 }
 
 // How a call is cut.  Pieces of 16 bytes where rows and groups fit them, else pairs; a team as narrow as covers the group with K pieces a
@@ -537,8 +596,8 @@ int aligned_to(std::initializer_list<const void*> ps, std::initializer_list<long
     return (int)(bits & (0 - bits));
 }
 // Shared memory of a CTA: the rows to come of so many streams, and behind them the CTA's sums of the parameters' gradients.
-template <typename T, int VEC, int K, bool kWhole, bool kAsync> size_t shared_bytes(const Plan& q, int streams, bool sums) {
-    const size_t rows = Rows<T, VEC, K, kWhole, kAsync>::kBytes * streams * q.block, room = sums ? 2 * 256 * VEC * sizeof(float) : 0;
+template <typename T, int VEC, int K, bool kWhole, bool kAsync> constexpr size_t shared_bytes(int block, int streams, bool sums) {
+    const size_t rows = Rows<T, VEC, K, kWhole, kAsync>::kBytes * streams * block, room = sums ? 2 * 256 * VEC * sizeof(float) : 0;
     return rows > room ? rows : room;
 }
 // `go` for the cut of a plan
@@ -586,7 +645,7 @@ template <typename T> int fwd(cudaStream_t st, Problem p, void* y) {
     return dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto team, auto gate) {
         const auto kern = group_norm_fwd_kernel<T, vec.value, k.value, whole.value, block.value, team.value, gate.value>;
         constexpr bool kAsync = vec.value == 8 && kAsyncRows<T, k.value, whole.value, block.value, true>;
-        const size_t smem = shared_bytes<T, vec.value, k.value, whole.value, kAsync>(q, 1 + gate.value, false);       // (48 KB at most)
+        const size_t smem = shared_bytes<T, vec.value, k.value, whole.value, kAsync>(q.block, 1 + gate.value, false);       // (48 KB at most)
         kern<<<q.grid, q.block, smem, st>>>(p, (T*)y);
         return cudaGetLastError() == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
     });
@@ -599,8 +658,18 @@ int bwd(cudaStream_t st, Problem p, const void* gy, void* dx, void* dgate, void*
     const int status = dispatch<T>(q, p, [&](auto vec, auto k, auto whole, auto block, auto team, auto gate) {
         const auto kern = group_norm_bwd_kernel<T, vec.value, k.value, whole.value, block.value, team.value, gate.value>;
         constexpr bool kAsync = vec.value == 8 && kAsyncRows<T, k.value, whole.value, block.value, false>;
-        const size_t smem = shared_bytes<T, vec.value, k.value, whole.value, kAsync>(q, 2 + gate.value, p.reduce);    // (36 KB at most)
-        kern<<<q.grid, q.block, smem, st>>>(p, (const T*)gy, (T*)dx, (T*)dgate, partial);
+        // (rows to come 36 KB at most, totals 16 to 64 KB for 256 threads, 64 KB for whole CTAs of 512)
+        constexpr size_t kTotals = kTotalBytes<k.value * vec.value / 2, !(block.value && k.value * vec.value > 8)>;
+        constexpr int kMost = block.value ? kMaxThreads : 256;
+        static DeviceOnce once;
+        if (!once.ok([&]() { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                         (int)(kTotals * kMost + shared_bytes<T, vec.value, k.value, whole.value, kAsync>(kMost, 2 + gate.value, !block.value))); }))
+            return (int)B200WKV_ELAUNCH;
+        const bool totals = partial != nullptr && p.rows > (long long)kChain * p.parallel;
+        const size_t ring = shared_bytes<T, vec.value, k.value, whole.value, kAsync>(q.block, 2 + gate.value, p.reduce), smem = ring + (totals ? kTotals * q.block : 0);
+        Problem pp = p;
+        pp.totals = totals ? (int)ring : -1;
+        kern<<<q.grid, q.block, smem, st>>>(pp, (const T*)gy, (T*)dx, (T*)dgate, partial);
         return cudaGetLastError() == cudaSuccess ? B200WKV_OK : B200WKV_ELAUNCH;
     });
     if (status != B200WKV_OK || !params) return status;
@@ -612,7 +681,7 @@ Problem problem(long long rows, int C, int groups, float eps, int act, const voi
                 int param_dtype, const void* gate, long long gate_stride) {
     const int f32 = param_dtype == B200WKV_F32;
     return {rows, C, groups, C / groups, act, eps, x, gate, x_stride, gate != nullptr ? gate_stride : 0, {weight, f32}, {bias, f32}, 0, 0, 0,
-            aligned_to({weight, bias}, {}, 1) >= 16, 0};
+            aligned_to({weight, bias}, {}, 1) >= 16, -1, 0};
 }
 }  // namespace
 

@@ -134,13 +134,22 @@ __device__ __forceinline__ float sum_of(F2 v) {
 }
 __device__ __forceinline__ F2 first_alone(F2 v) { return make_f2(parts(v).x, 0.f); }
 
-// act(z), and its derivative where it is asked for
+// act(z), and its derivative where it is asked for.  Below -87 silu is what it is there, -1.5e-36: sigmoid's least value, 2^-126, times the z of a
+// closed gate, which may be the type's lowest number, is none of the function's values (-4).  -inf counts as closed too.
 template <typename T, int kAct> __device__ __forceinline__ void activate(F2 z, F2& p, F2& dp) {
     if (kAct == B200WKV_ACT_NONE) { p = z; dp = both(1.f); return; }
     F2 s, r;
-    sigmoid_pair<T>(z, s, r);
-    p = kAct == B200WKV_ACT_SIGMOID ? s : mul2(z, s);
-    dp = kAct == B200WKV_ACT_SIGMOID ? mul2(s, r) : mul2(s, fma2(z, r, both(1.f)));
+    if (kAct == B200WKV_ACT_SIGMOID) {
+        sigmoid_pair<T>(z, s, r);
+        p = s;
+        dp = mul2(s, r);
+    } else {
+        const float2 t = parts(z);
+        z = make_f2(max_nan(t.x, -87.f), max_nan(t.y, -87.f));
+        sigmoid_pair<T, true>(z, s, r);
+        p = mul2(z, s);
+        dp = mul2(s, fma2(z, r, both(1.f)));
+    }
 }
 
 // Where a thread's team works: group g, rows first, first + parallel, ...; none of them where `at_work` is false.  A warp has as many teams as fit

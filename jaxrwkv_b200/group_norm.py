@@ -87,7 +87,8 @@ def group_norm_act(x, weight, bias, groups, gate=None, activation="silu", eps=1e
     over each row's ``groups`` groups of ``C // groups`` consecutive channels (at most 8192), then ``act(n)``, or
     ``n * act(gate)`` where a gate of x's shape is given.
 
-    ``activation`` is "none", "sigmoid" or "silu"; ``weight`` and ``bias`` are (C,), float32 or bfloat16, each may be None.
+    ``activation`` is "none", "sigmoid" or "silu", which is 0 far below zero and of -inf too: a closed gate lets nothing through.
+    ``weight`` and ``bias`` are (C,), float32 or bfloat16, each may be None.
     ``x`` and ``gate`` are read where they lie as long as their channels are adjacent and their rows evenly spaced (parts of
     a projection's rows).  The arithmetic is float32, results are rounded once.
     """

@@ -73,7 +73,9 @@ class _GatedBwd(torch.autograd.Function):
             xr, fr = _rows(x, (B, T, C)), _rows(f, (B, T, C))
             length, new_starts = _flag_bytes(length, new_starts, lead, (T,), x.device)
             gs = None if gs is None else gs.to(torch.float32).contiguous()
-            gy = _cotangent(gy, x.dtype)
+            gy, residual = _cotangent(gy, x.dtype), _cotangent(residual, torch.uint8)
+            if residual.numel() != lib.b200wkv_gated_residual_bytes(B, T, C):
+                raise _lib.B200WKVError("gated_recurrence: the residual is another call's")
             dx, df = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
             ds = torch.empty(lead + (C,), dtype=torch.float32, device=x.device)
             _lib.check(lib.b200wkv_gated_bwd(_stream(), _lib.dtype_code(x.dtype), gate, B, T, C, _ptr(xr), xr.stride(0), xr.stride(1),
@@ -91,7 +93,7 @@ class _GatedBwd(torch.autograd.Function):
 
     @staticmethod
     def vmap(info, in_dims, x, f, length, new_starts, residual, gs, gy, gate):
-        x, f, length, new_starts, gs, gy = _batched(info.batch_size, (x, f, length, new_starts, gs, gy), in_dims[:4] + in_dims[5:7])
+        x, f, length, new_starts, residual, gs, gy = _batched(info.batch_size, (x, f, length, new_starts, residual, gs, gy), in_dims[:7])
         return _GatedBwd.apply(x, f, length, new_starts, residual, gs, gy, gate), (0, 0, 0)
 
 
@@ -112,7 +114,8 @@ class _Gated(torch.autograd.Function):
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             s_out = torch.empty(lead + (C,), dtype=torch.float32, device=x.device)
             rbytes = lib.b200wkv_gated_residual_bytes(B, T, C)
-            residual = torch.empty(rbytes, dtype=torch.uint8, device=x.device)
+            # by sequences, so that a call under vmap hands each instance its own, and a backward call sees whose they are
+            residual = torch.empty(lead + (rbytes // B,), dtype=torch.uint8, device=x.device)
             _lib.check(lib.b200wkv_gated_fwd(_stream(), code, gate, B, T, C, _ptr(xr), xr.stride(0), xr.stride(1), _ptr(fr), fr.stride(0),
                                              fr.stride(1), _ptr(sr), _ptr(length), _ptr(new_starts), _ptr(out), _ptr(s_out),
                                              _ptr(residual), rbytes))
@@ -139,7 +142,7 @@ class _Gated(torch.autograd.Function):
     def vmap(info, in_dims, x, f, s, length, new_starts, gate):
         args = _batched(info.batch_size, (x, f, s, length, new_starts), in_dims[:5])
         s_out, out, residual = _Gated.apply(*args, gate)
-        return (s_out, out, residual), (0, 0, None)
+        return (s_out, out, residual), (0, 0, 0)
 
 
 def gated_recurrence(x, f, s, length=None, new_starts=None, gate="sigmoid"):

@@ -12,7 +12,7 @@ Host side of ``b200wkv_gated_{fwd,bwd,step}``.  Arrays are CUDA ``torch`` tensor
 import torch
 
 from . import _lib
-from .rwkv7 import _cotangent, _ptr, _stream, _vmap_front
+from .rwkv7 import _cotangent, _ptr, _stream, _vmap_flags, _vmap_front
 
 GATES = {"sigmoid": 0, "decay": 1}
 
@@ -93,8 +93,14 @@ class _GatedBwd(torch.autograd.Function):
 
     @staticmethod
     def vmap(info, in_dims, x, f, length, new_starts, residual, gs, gy, gate):
-        x, f, length, new_starts, residual, gs, gy = _batched(info.batch_size, (x, f, length, new_starts, residual, gs, gy), in_dims[:7])
+        length, new_starts = _vmap_flags(length, new_starts, in_dims[2:4], _rank(x, in_dims[0]))
+        x, f, residual, gs, gy = _batched(info.batch_size, (x, f, residual, gs, gy), in_dims[:2] + in_dims[4:7])
         return _GatedBwd.apply(x, f, length, new_starts, residual, gs, gy, gate), (0, 0, 0)
+
+
+def _rank(x, dim):
+    """Leading axes of an instance's x (..., T, C)."""
+    return x.dim() - 2 - (dim is not None)
 
 
 def _batched(n, xs, dims):
@@ -140,8 +146,9 @@ class _Gated(torch.autograd.Function):
 
     @staticmethod
     def vmap(info, in_dims, x, f, s, length, new_starts, gate):
-        args = _batched(info.batch_size, (x, f, s, length, new_starts), in_dims[:5])
-        s_out, out, residual = _Gated.apply(*args, gate)
+        length, new_starts = _vmap_flags(length, new_starts, in_dims[3:5], _rank(x, in_dims[0]))
+        x, f, s = _batched(info.batch_size, (x, f, s), in_dims[:3])
+        s_out, out, residual = _Gated.apply(x, f, s, length, new_starts, gate)
         return (s_out, out, residual), (0, 0, 0)
 
 

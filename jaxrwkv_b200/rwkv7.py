@@ -142,6 +142,19 @@ def _vmap_front(n, xs, dims, required):
     return out
 
 
+def _vmap_flags(length, new_starts, dims, rank):
+    """Flags of a call under vmap, whose instances have ``rank`` leading axes: a mapped one with its mapped axis in front of those
+    of its instances that it has and, as axes of length 1, those that it has not; one that is not mapped as it is, which the
+    instances share as their leading axes do."""
+    out = []
+    for x, d, full in zip((length, new_starts), dims, (rank, rank + 1)):
+        if d is not None:
+            x = x.movedim(d, 0)
+            x = x.reshape(x.shape[:1] + (1,) * (full + 1 - x.dim()) + x.shape[1:])
+        out.append(x)
+    return out
+
+
 class _WKV7Bwd(torch.autograd.Function):
     """The ``wkv7-bwd`` call as its own function so that it has a batching rule too
     (rwkv7.py:434-440).  Not differentiable a second time."""

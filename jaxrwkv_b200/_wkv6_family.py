@@ -10,7 +10,7 @@ constant decay) are never batched, as under ``jax.vmap(..., in_axes=None)``.
 import torch
 
 from . import _lib
-from .rwkv7 import _ptr, _stream, _cotangent, _flatten_lead, _bcast_flags, _vmap_front
+from .rwkv7 import _ptr, _stream, _cotangent, _flatten_lead, _bcast_flags, _vmap_flags, _vmap_front
 
 
 def _expand_hn(x, H, N, dtype):
@@ -109,7 +109,8 @@ def _make_functions(version):
             r, k, v = _vmap_front(n, (r, k, v), in_dims[:3], (True,) * 3)
             if per_token:
                 w, = _vmap_front(n, (w,), in_dims[3:4], (True,))
-            s, length, new_starts = _vmap_front(n, (s, length, new_starts), in_dims[5:8], (True, False, False))
+            s, = _vmap_front(n, (s,), in_dims[5:6], (True,))
+            length, new_starts = _vmap_flags(length, new_starts, in_dims[6:8], k.dim() - 4)
             gs_out, gy = _vmap_front(n, (gs_out, gy), in_dims[9:], (False, False))
             outs = Bwd.apply(r, k, v, w, u, s, length, new_starts, residual, gs_out, gy)
             # gradients of the shared operands are already summed over the batch
@@ -148,7 +149,8 @@ def _make_functions(version):
             r, k, v = _vmap_front(n, (r, k, v), in_dims[:3], (True,) * 3)
             if per_token:
                 w, = _vmap_front(n, (w,), in_dims[3:4], (True,))
-            s, length, new_starts = _vmap_front(n, (s, length, new_starts), in_dims[5:8], (True, False, False))
+            s, = _vmap_front(n, (s,), in_dims[5:6], (True,))
+            length, new_starts = _vmap_flags(length, new_starts, in_dims[6:8], k.dim() - 4)
             new_s, out, residual = Fwd.apply(r, k, v, w, u, s, length, new_starts)
             return (new_s, out, residual), (0, 0, None)
 

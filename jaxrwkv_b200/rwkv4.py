@@ -9,7 +9,7 @@ operator (``w`` is the raw decay parameter; ``-exp(w)`` is applied here, rwkv4.p
 import torch
 
 from . import _lib
-from .rwkv7 import _ptr, _stream, _vmap_front
+from .rwkv7 import _ptr, _stream, _vmap_flags, _vmap_front
 
 
 def batched_wkv4_fwd(k, v, w_neg, time_first, s, length, new_starts, B, need_residual=True):
@@ -94,8 +94,10 @@ class _WKV4Bwd(torch.autograd.Function):
         n = info.batch_size
         if in_dims[2] is not None or in_dims[3] is not None:
             raise _lib.B200WKVError("wkv4 under vmap: w and time_first cannot be batched")     # rwkv4.py:362-363
+        rank = k.dim() - 2 - (in_dims[0] is not None)
         k, v = _vmap_front(n, (k, v), in_dims[:2], (False, False))
-        s, length, new_starts = _vmap_front(n, (s, length, new_starts), in_dims[4:7], (False, False, False))
+        s, = _vmap_front(n, (s,), in_dims[4:5], (False,))
+        length, new_starts = _vmap_flags(length, new_starts, in_dims[5:7], rank)
         gs_new, gy = _vmap_front(n, (gs_new, gy), in_dims[8:], (False, False))
         outs = _WKV4Bwd.apply(k, v, w, u, s, length, new_starts, residual, gs_new, gy)
         return outs, (0, 0, None, None, 0)
@@ -133,8 +135,10 @@ class _WKV4(torch.autograd.Function):
         n = info.batch_size
         if in_dims[2] is not None or in_dims[3] is not None:
             raise _lib.B200WKVError("wkv4 under vmap: w and time_first cannot be batched")
+        rank = k.dim() - 2 - (in_dims[0] is not None)
         k, v = _vmap_front(n, (k, v), in_dims[:2], (False, False))
-        s, length, new_starts = _vmap_front(n, (s, length, new_starts), in_dims[4:7], (False, False, False))
+        s, = _vmap_front(n, (s,), in_dims[4:5], (False,))
+        length, new_starts = _vmap_flags(length, new_starts, in_dims[5:7], rank)
         new_s, out, residual = _WKV4.apply(k, v, w, u, s, length, new_starts)
         return (new_s, out, residual), (0, 0, None)
 

@@ -184,7 +184,8 @@ class _WKV7Bwd(torch.autograd.Function):
     @staticmethod
     def vmap(info, in_dims, r, w, k, v, a, b, s, length, new_starts, residual, gs_out, gy):
         n = info.batch_size
-        args = _vmap_front(n, (r, w, k, v, a, b, s, length, new_starts), in_dims[:9], (True,) * 7 + (False, False))
+        flags = _vmap_flags(length, new_starts, in_dims[7:9], k.dim() - 4)
+        args = _vmap_front(n, (r, w, k, v, a, b, s), in_dims[:7], (True,) * 7) + flags
         gs_out, gy = _vmap_front(n, (gs_out, gy), in_dims[10:], (False, False))
         outs = _WKV7Bwd.apply(*args, residual, gs_out, gy)
         return outs, (0,) * 7
@@ -218,10 +219,10 @@ class _WKV7(torch.autograd.Function):
     @staticmethod
     def vmap(info, in_dims, r, w, k, v, a, b, s, length, new_starts):
         """Batching rule (rwkv7.py:419-431): the seven tensors must be batched, ``length`` and
-        ``new_starts`` are broadcast when they are not; the new axis becomes one more leading
+        ``new_starts`` are shared when they are not; the new axis becomes one more leading
         batch axis, which ``forward`` flattens — so nesting works to any depth."""
-        args = _vmap_front(info.batch_size, (r, w, k, v, a, b, s, length, new_starts), in_dims,
-                           (True,) * 7 + (False, False))
+        flags = _vmap_flags(length, new_starts, in_dims[7:9], k.dim() - 4)
+        args = _vmap_front(info.batch_size, (r, w, k, v, a, b, s), in_dims[:7], (True,) * 7) + flags
         new_s, out, residual = _WKV7.apply(*args)
         return (new_s, out, residual), (0, 0, None)
 

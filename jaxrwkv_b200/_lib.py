@@ -18,6 +18,7 @@ _SZ = ctypes.c_size_t
 _U = ctypes.c_uint
 _L = ctypes.c_longlong
 _F = ctypes.c_float
+INT_MAX = (1 << 31) - 1          # ctypes hands on the low 32 bits of what is larger, without a word
 
 # name -> (restype, argtypes); must list every symbol the header declares
 PROTOTYPES = {

@@ -34,8 +34,10 @@ def _check_operands(x, f, s, state_shape):
         raise _lib.B200WKVError("gated_recurrence: the state is kept in float32")
     if x.shape != f.shape or tuple(s.shape) != tuple(state_shape):
         raise _lib.B200WKVError(f"gated_recurrence: shapes do not fit: x {tuple(x.shape)}, f {tuple(f.shape)}, s {tuple(s.shape)}")
-    if x.numel() == 0:
-        raise _lib.B200WKVError("gated_recurrence: every dimension must be at least 1")
+    if x.dim() == 0 or x.numel() == 0:
+        raise _lib.B200WKVError("gated_recurrence: there must be channels, and every dimension must be at least 1")
+    if x.numel() // x.shape[-1] > _lib.INT_MAX or x.shape[-1] > _lib.INT_MAX:          # (the library counts both in 32 bits)
+        raise _lib.B200WKVError("gated_recurrence: more tokens or channels than 32 bits count")
     return _lib.dtype_code(x.dtype)
 
 

@@ -23,6 +23,8 @@ def _check_operands(x, weight, bias, gate, groups):
     if x.dim() < 1 or x.numel() == 0:
         raise _lib.B200WKVError("group_norm_act: every dimension must be at least 1")
     C = x.shape[-1]
+    if C > _lib.INT_MAX:                         # (the library counts them in 32 bits)
+        raise _lib.B200WKVError("group_norm_act: more channels than 32 bits count")
     if not (isinstance(groups, int) and groups >= 1 and C % groups == 0 and C // groups <= MAX_GROUP):
         raise _lib.B200WKVError(f"group_norm_act: {C} channels cannot be cut into {groups} groups of at most {MAX_GROUP}")
     if gate is not None and (gate.dtype != x.dtype or gate.shape != x.shape):

@@ -12,13 +12,15 @@
 //   3. walks the segment from that state and writes the outputs.
 // Where there are sequences enough for the device, a CTA has one to itself and step 2 is a box that the warp in front fills when it
 // has walked its segment (Mail): no warp waits for another but for that.  Forward / backward of B=8, T=4096, C=2048, bf16, sigmoid: 72 / 118 us,
-// 0.94 / 0.92 of the measured copy rate; 256 CTAs on 296 places.  A segment's way through the chain takes 333 cycles (265 backward), which
+// 0.94 / 0.92 of the measured copy rate (ncu's clock; between events around a call whose operands are not in L2, as the figures further
+// down, 80 / 131); 256 CTAs on 296 places.  A segment's way through the chain takes 333 cycles (265 backward), which
 // is what bounds a long sequence then: 11 ns a token.
 // Where there are fewer, a cluster of up to eight CTAs shares a sequence, tile by tile.  The recurrence is associative: a stretch of
 // tokens acts on the state entering it as h -> A h + b.  The warps reduce their segments to (A, b), the last one sends the whole tile's to
 // every CTA of the cluster (st.async onto an mbarrier there), and everyone carries the state over all tiles of the round: one hop,
-// whatever the size of the cluster.  One sequence of 32768 tokens, C=2048: 96 us in 32 clusters of eight, 0.65 of the copy rate; 48 % of issue slots,
-// the rest latency of a round's barrier and hop, which two CTAs an SM hide in part.
+// whatever the size of the cluster.  One sequence of 32768 tokens, C=2048: 96 us in 32 clusters of eight, 0.65 of the copy rate; 48 % of issue slots.
+// A round is a chain of steps that wait for one another (gates, summary, barrier, the joins of eight segments, hop, the joins of eight CTAs, walk),
+// which two CTAs an SM hide in part; the hop is 8 us of the 96.
 // Segments of 16 tokens and a pair of channels a lane are what 128 registers hold; with 8 tokens the work around a segment makes the forward
 // 125 us instead of 82, with 16 warps a CTA 107 (both measured in the form with barriers).
 //
@@ -644,7 +646,8 @@ struct Residency {
 // clusters in front of it; the smaller of equals.  One CTA alone takes half of a cluster's time for a round.  Forward / backward in us with one CTA a
 // sequence and with clusters, bf16: B=4, T=1024, C=2048 20 / 29 and 25 / 31 (of two); B=16, T=512, C=768 16 / 22 and 27 / 33 (two); B=2, T=8192,
 // C=1024 98 / 156 and 35 / 51 (eight); B=1, T=2000, C=2560 30 and 21 (six); B=8, T=1024, C=1001 25 / 37 and 30 / 41 (two); fp32, B=4, T=2048, C=2048
-// 43 / 64 and 45 / 80 (two); B=8, T=2048, C=1001 49 / 73 and 55 / 107 (two); the rule's miss: B=3, T=1023, C=1001 backward 37 and 33 (two).
+// 43 / 64 and 45 / 80 (two); B=8, T=2048, C=1001 49 / 73 and 55 / 107 (two); the rule's miss: B=3, T=1023, C=1001 backward 37 and 33 (two; all of these
+// with the sigmoid gate, the decay gate takes up to 10 % more).
 // units: 64 channels of a sequence each; tiles: of one of them.
 int ranks_of(const int* alone, const int* resident, long long units, int tiles) {
     constexpr double kAlone = 0.5;

@@ -11,10 +11,12 @@
 // CTA where the group is wider than that.  The row's values stay in registers from the mean over the centred squares to the
 // result.  A team keeps its group from row to row, so that weight and bias are read once and their gradients are added up in
 // registers; they leave as partial rows, which a second kernel adds in a fixed order.
-// 32768 rows of 32 groups of 64 channels, bf16, silu of a gate: forward 61 us, 1.02 of the measured copy rate; backward 110 us, 0.95, and
-// 4 us for the sums behind it.  Groups that are no power of two of pieces leave lanes idle (24 groups of 72: 5 of 32) and take longer sums: 20
-// groups of 80 reach 0.73 and 0.71 of the copy rate, bound by issue slots.  Single elements, as of 32 groups of 61, reach 0.40 and 0.41, bound by
-// the number of loads.
+// 32768 rows of 32 groups of 64 channels, bf16, silu of a gate: forward 60 us, 1.04 of the measured copy rate; backward 110 us, 0.94, and
+// 4 us for the sums behind it (ncu's clock; between events around a call whose operands are not in L2, as the figures below, 74 and 125 in all).
+// Groups that are no power of two of pieces leave lanes idle (24 groups of 72: 5 of 32) and take longer sums: 20 groups of 80 reach 0.70 and
+// 0.69 of the copy rate, 32 of 40 0.64 and 0.71.  Single elements, as of 32 groups of 61, reach 0.40 and 0.39, bound by the number of loads.
+// Backward of wide groups: 8 of 512 0.66 gated and 0.48 not, one of 2048 0.49 and 0.31 (eight warps an SM, one row ahead, in whole CTAs
+// four barriers a row), one of 5120 0.27 and one of 4097 0.06 (the registers of 16 channels a thread spill).
 #include <initializer_list>
 #include <type_traits>
 
@@ -574,8 +576,11 @@ Plan plan_of(Problem& p, int element, int aligned, bool forward) {
     p.reduce = p.G * 4 <= teams;
     p.per_cta = p.reduce ? teams / p.G * p.G : teams;
     const long long all = p.rows * p.G;                  // rows of groups
-    // as many threads as the device has room for: a backward keeps its parameters' sums, so its CTAs are no more than are resident (fp32, 16777
-    // rows of 2 groups of 1000, with one too many: 219 us, else 170)
+    // As many threads as an SM takes at most, and no more rows at a time than partial rows.  In the forward that is neither what a kernel's registers let in (two
+    // to four CTAs of 256) nor a limit of its own, but the waves that it makes happen to suit the training size: without the cap 32768 rows of 32 groups of 64
+    // take 76.6 instead of 73.8 us, of 5 groups of 128 28.9 instead of 32.8, of 20 groups of 80 65.6 instead of 68.4.
+    // A backward keeps its parameters' sums, so its CTAs are no more than are resident (fp32, 16777 rows of 2 groups of 1000, with one too many:
+    // 219 us, else 170).
     const int elements = q.vec * q.k;
     const int threads = forward ? 2048 : p.team > 32 ? 512 : 256 * bwd_ctas(elements, elements * (q.whole ? element : 4), p.gate != nullptr), ctas = threads > q.block ? threads / q.block : 1;
     const long long most_ctas = (long long)sm_count_of_current_device() * (ctas < 32 ? ctas : 32);

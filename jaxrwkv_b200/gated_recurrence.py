@@ -179,6 +179,7 @@ def gated_recurrence_step(x, f, s, new_starts=None, length=None, gate="sigmoid",
     """One token of :func:`gated_recurrence` without autograd: ``x``, ``f`` and the float32 state ``s`` are (..., C),
     ``length`` (...), ``new_starts`` (...) or (..., 1).  Returns ``(s_out, out)``; a row of length 0 keeps its state and has its output all the same.  With
     ``inplace`` the state is updated where it lies (rows of a wider container may have any distance) and ``s_out`` is ``s``.
+    There is no batching rule for ``torch.func.vmap``: leading axes are what it takes instead.
     """
     code = _gate_code(gate)
     if x.is_cuda:

@@ -298,7 +298,7 @@ template <int kAhead, bool kAsync> __device__ __forceinline__ void arrived() {
 // sum); else without, where the registers of a whole CTA have spilled and want the L1 cache (5120 channels: a pass 329 us, with 392).  dweight and
 // dbias of 32768 rows of 32 groups of 64, bf16 streams: 1.1e-7 and 1.0e-7 off (2-norm) instead of 2.2e-7, the terms alone are 0.8e-7 and 0.5e-7;
 // with 8 rows at a time 1.0e-7 and 0.9e-7, and 2 us more.  The pass through autograd 187 -> 185 us, without a gate 144 -> 153,
-// 8192 rows of 5120 channels 317 -> 329, 16384 rows of 2048 148 -> 154, fp32 rows of 2 groups of 1000 246 -> 241, others within 2.5 %.
+// 8192 rows of 5120 channels 317 -> 329, 16384 rows of 2048 148 -> 154, fp32 rows of 2 groups of 1000 246 -> 241, others within 3 %.
 template <int kPairs, bool kExact, int kThreads> struct Totals {
     struct alignas(kExact ? 16 : 8) Sum { F2 v[kExact ? 2 : 1]; };       // the sum, and what it is too large by
     Sum* at;
